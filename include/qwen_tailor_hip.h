@@ -244,6 +244,58 @@ int qt_blit_batch(void* const* dst, const void* const* src, const long* meta, in
 /* qt_blit_batch with jobs that fill: where src[k] is null the rows of job k become zeros (its s0 and sstride are not used). */
 int qt_blit_fill_batch(void* const* dst, const void* const* src, const long* meta, int count, qt_stream_t stream);
 
+/* ---- several branches of a sequence: drafted trees and beams.  No counterpart in the reference, which verifies chains. ----------
+ *
+ * A drafted tree: sequence b drafts M tokens (1 <= M <= 64), parents [B,M] int32 is the index of a token's parent among them, smaller than its own,
+ * or -1: a child of the sequence's last committed token (anything else counts as -1).  A sequence that drafts fewer pads its rows with
+ * -1; no other token sees them.  Row b*M + j is token j.  Values of a token that are not finite reach no row that does not descend from it;
+ * the token's own row and its descendants' become NaN.  Output rows of skipped sequences are zero.
+ *
+ * qt_gdn_tree_step: the GatedDeltaNet step of the M tokens, every token from the state and conv window that its parent leaves (the outputs of
+ * qt_gdn_verify_step for a chain, up to the order of sums).  proj [B*M,8224]; pools, slots and pos as for qt_gdn_decode_step; the pools are only read and
+ * no token's state is stored (qt_tree_commit advances them).  y [B*M,2048].  k and q of a token take part as bf16, the state as two
+ * bf16 terms (2^-17 of an element); a |v| of 2^100 or more counts as not finite. */
+int qt_gdn_tree_step(const void* proj, const void* conv_pool, const void* conv_w, const float* A_log, const float* dt_bias, const float* ssm_pool,
+                     const int32_t* slots, const int32_t* pos, const int32_t* parents, void* y, int B, int M, int n_slots, qt_stream_t stream);
+
+/* Attention of the M tokens: token j sees the pool keys below pos[b], its ancestors' new keys and its own.  q, k_new, v_new, pools, slots, pos and out as
+ * for qt_gqa_attn_decode; new row j is appended at pos[b] + j (a sequence with pos[b] + M > Lmax is skipped).  B <= 1024.  Workspace of
+ * at least qt_gqa_tree_workspace_bytes(B, M) bytes, 16-byte aligned; nothing in it has to be set. */
+long qt_gqa_tree_workspace_bytes(int B, int M);
+int qt_gqa_tree_attn(const void* q, const void* k_new, const void* v_new, void* Kp, void* Vp, const int32_t* slots, const int32_t* pos,
+                     const int32_t* parents, void* out, void* workspace, long workspace_bytes, int B, int M, int Lmax, int n_slots, qt_stream_t stream);
+/* The attention half of a full-attention layer around it, as qt_gqa_attn_layer_decode: token j sits at position pos[b] + the number of its ancestors (its
+ * rotary angle), its K / V row at pos[b] + j.  rope_table may be null (table_positions 0): rows beyond it evaluate their own pairs. */
+long qt_gqa_tree_layer_workspace_bytes(int B, int M);
+int qt_gqa_tree_layer(const void* qkv, const void* q_norm, const void* k_norm, const void* rope_table, int table_positions, void* Kp, void* Vp,
+                      const int32_t* slots, const int32_t* pos, const int32_t* parents, void* out, void* workspace, long workspace_bytes, int B, int M,
+                      int Lmax, int n_slots, float eps, qt_stream_t stream);
+
+/* The accepted path of each tree becomes part of its sequence, in all layers: path [B,D] (1 <= D <= 64) the indices among the M tokens from the root down,
+ * count [B] how many of them (<= 0: nothing happens; more than D count as D).  For each of the n_gdn recurrent layers (tables of
+ * device pointers in host memory: proj [B*M,8224], conv_pool, conv_w, A_log, dt_bias, ssm_pool) the state advances in place through those tokens with the
+ * bits of as many calls of qt_gdn_decode_step, and the new window goes to conv buffer (pos + count) & 1.  For each of the n_kv K / V pools
+ * [n_slots,2,Lmax,256] rows pos + path[j] move to pos + j.  The sequence then holds pos + count tokens.  With K / V pools a sequence with pos < 0 or
+ * pos + M > Lmax is skipped, as by the attention. */
+int qt_tree_commit(const void* const* proj, void* const* conv_pool, const void* const* conv_w, const float* const* A_log, const float* const* dt_bias,
+                   float* const* ssm_pool, int n_gdn, void* const* kv_pool, int n_kv, const int32_t* slots, const int32_t* pos, const int32_t* path,
+                   const int32_t* count, int B, int M, int D, int n_slots, int Lmax, qt_stream_t stream);
+
+/* Beam search's selection.  logits: G sequences x W beams x V (dtype 0 bf16, 1 fp16, 2 f32), element strides stride_g, stride_w, the vocabulary contiguous;
+ * scores [G,W] the beams' log-probabilities.  Candidate (w, t) scores scores[w] + logits[w][t] - log sum exp logits[w]; the n largest of a
+ * sequence go to out_scores, out_parents (w) and out_tokens (t) [G,n] in falling order, equal ones by the lower w V + t.  A candidate whose score is -inf
+ * or NaN is none; places that are left over get -inf, -1, -1.  W, n <= 64, G W <= 65535.  Workspace: qt_beam_select_workspace_bytes, 16-byte
+ * aligned. */
+long qt_beam_select_workspace_bytes(long G, int W, int V, int n, int elem_size);
+int qt_beam_select(const void* logits, int dtype, long stride_g, long stride_w, const float* scores, float* out_scores, int32_t* out_parents,
+                   int32_t* out_tokens, void* workspace, long workspace_bytes, int G, int W, int V, int n, qt_stream_t stream);
+
+/* The beams' states follow: for all beams at once the state in slot slots[g][w] becomes that of slot slots[g][parents[g][w]], in place (parents [G,W]; a beam
+ * whose parent is itself or none stays as it is).  Of each layer the recurrent state, the conv buffer pos[g] & 1, and the K / V rows start[g] .. pos[g] -
+ * 1 (rows before start are common to the beams).  The slots of a call are different from each other, but for those of beams that stay as they are.  W <= 32. */
+int qt_beam_reorder(float* const* ssm_pool, void* const* conv_pool, int n_gdn, void* const* kv_pool, int n_kv, const int32_t* slots,
+                    const int32_t* parents, const int32_t* start, const int32_t* pos, int G, int W, int n_slots, int Lmax, qt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,6 +50,12 @@ _SIGS = {
     "qt_rms_rows": [_vp, _vp, _vp, _i, _i, _f, _vp],
     "qt_fused_gemv_rms": [_vp, _vp, _vp, _f, _vp, _vp, _i, _i, _i, _i, _vp],
     "qt_fused_gemv": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
+    "qt_gdn_tree_step": [_vp] * 10 + [_i, _i, _i, _vp],
+    "qt_gqa_tree_attn": [_vp] * 10 + [_l] + [_i] * 4 + [_vp],
+    "qt_gqa_tree_layer": [_vp] * 4 + [_i] + [_vp] * 7 + [_l] + [_i] * 4 + [_f, _vp],
+    "qt_tree_commit": [_vp] * 6 + [_i, _vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp],
+    "qt_beam_select": [_vp, _i, _l, _l] + [_vp] * 5 + [_l] + [_i] * 4 + [_vp],
+    "qt_beam_reorder": [_vp, _vp, _i, _vp, _i] + [_vp] * 4 + [_i] * 4 + [_vp],
 }
 
 
@@ -70,6 +76,9 @@ def lib():
         for name in ("qt_gdn_chunk_ops_bytes", "qt_gdn_chunk_u_bytes", "qt_gdn_chunk_gc_bytes", "qt_gdn_chunk_snap_bytes",
                      "qt_gdn_chunk_flag_bytes", "qt_gqa_prefill_workspace_bytes"):
             getattr(L, name).argtypes, getattr(L, name).restype = [_i], ctypes.c_long
+        for name in ("qt_gqa_tree_workspace_bytes", "qt_gqa_tree_layer_workspace_bytes"):
+            getattr(L, name).argtypes, getattr(L, name).restype = [_i] * 2, ctypes.c_long
+        L.qt_beam_select_workspace_bytes.argtypes, L.qt_beam_select_workspace_bytes.restype = [_l] + [_i] * 4, ctypes.c_long
         L.qt_gqa_prefill_workspace_bytes_for.argtypes, L.qt_gqa_prefill_workspace_bytes_for.restype = [_i] * 3, ctypes.c_long
         _lib = L
     return _lib
@@ -95,7 +104,7 @@ class _Host:
 
     FUNCTIONS = ("rms_rows", "fused_gemv", "gated_norm", "decode_step", "decode_step_gnorm", "verify_step", "deltanet", "attn_b", "attn_layer_b",
                  "sdpa", "qkv_prep", "out_gate", "conv_prep", "phase_a", "phase_b", "phase_b_norm", "gdn_core", "blit_batch", "pools_load",
-                 "cache_restore")
+                 "cache_restore", "deltanet_bt", "attn_bt", "attn_layer_bt", "tree_commit", "beam_select", "beam_reorder")
 
     def __getattr__(self, name):
         if name not in self.FUNCTIONS:

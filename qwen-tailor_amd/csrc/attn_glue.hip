@@ -9,7 +9,7 @@
 // theta = float(pos) * freq_i with freq_i = float(1e7^(-2 i / 64)); cos / sin = the double-precision libm values rounded to
 // float; y1' = BF(y1 * c - y2 * s), y2' = BF(y1 * s + y2 * c), each product and the sum rounded to float separately;
 // gate: BF(o * sigmoid_bf16(g)) with the bf16 sigmoid of the GatedDeltaNet path (qwen35/mslib.py:16-20).
-#include "qt_common.h"
+#include "tree.h"
 
 using namespace qt;
 
@@ -35,11 +35,13 @@ __constant__ float rope_freq[ROPE_DIM / 2] = {
 // us with a workgroup per row, 8 bytes per lane and the sums over 64 lanes through LDS; now 5.4 / 8.6 / 13.9 / 25.0 us (4 TB/s).
 // Nontemporal stores would take another 1 us off this kernel at 2048 rows, and cost the attention kernel that reads q next 18 us
 // at 8192.
+// TREE: row r = b * M + j is token j of a tree and sits at position pos[b] + its depth in the tree (the number of its ancestors).
+template <bool TREE>
 __global__ __launch_bounds__(256) void attn_qkv_prep_kernel(const bf16_t* __restrict__ qkv, const bf16_t* __restrict__ q_norm,
                                                             const bf16_t* __restrict__ k_norm, const int* __restrict__ pos,
                                                             bf16_t* __restrict__ q, bf16_t* __restrict__ k, bf16_t* __restrict__ v,
                                                             long R, int M, float eps, const float2* __restrict__ table,
-                                                            int table_positions) {
+                                                            int table_positions, const int* __restrict__ parents) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4), aligned(8)));      // the entry points ask for 8-byte alignment only
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     __shared__ __align__(16) float2 cs_s[4][ROPE_DIM / 2];
@@ -57,7 +59,12 @@ __global__ __launch_bounds__(256) void attn_qkv_prep_kernel(const bf16_t* __rest
         wn[0][hf] = *reinterpret_cast<const u32x4*>(q_norm + 8 * c + 128 * hf);
         wn[1][hf] = *reinterpret_cast<const u32x4*>(k_norm + 8 * c + 128 * hf);
     }
-    const int ip = pos[(unsigned)r / (unsigned)M] + (int)((unsigned)r % (unsigned)M);
+    int ip = pos[(unsigned)r / (unsigned)M];
+    const int tok = (int)((unsigned)r % (unsigned)M);
+    if constexpr (TREE)
+        ip += __builtin_amdgcn_readlane(__popcll(tree_ancestors(tree_parent(parents + (r - tok), lane, M), lane)), tok) - 1;
+    else
+        ip += tok;
     if (lane < ROPE_DIM / 2) {
         if (ip >= 0 && ip < table_positions) {                   // (table_positions = 0 without a table)
             cs_s[w][lane] = table[(size_t)ip * (ROPE_DIM / 2) + lane];
@@ -181,15 +188,26 @@ int qt_attn_qkv_prep_table(const void* qkv, const void* q_norm, const void* k_no
     if (R == 0) return QT_OK;
     for (const void* p : {qkv, q_norm, k_norm, rope_table, (const void*)q, (const void*)k, (const void*)v})
         if (reinterpret_cast<uintptr_t>(p) & 7u) return QT_ERR_ALIGN;
-    hipLaunchKernelGGL(attn_qkv_prep_kernel, dim3((unsigned)((R + 3) / 4)), dim3(256), 0, stream, (const bf16_t*)qkv, (const bf16_t*)q_norm,
+    hipLaunchKernelGGL(attn_qkv_prep_kernel<false>, dim3((unsigned)((R + 3) / 4)), dim3(256), 0, stream, (const bf16_t*)qkv, (const bf16_t*)q_norm,
                        (const bf16_t*)k_norm, pos, (bf16_t*)q, (bf16_t*)k, (bf16_t*)v, R, M, eps, (const float2*)rope_table,
-                       rope_table ? table_positions : 0);
+                       rope_table ? table_positions : 0, (const int*)nullptr);
     QT_CHECK_LAUNCH();
     return QT_OK;
 }
 int qt_attn_qkv_prep(const void* qkv, const void* q_norm, const void* k_norm, const int32_t* pos, void* q, void* k, void* v, long R,
                      int M, float eps, hipStream_t stream) {
     return qt_attn_qkv_prep_table(qkv, q_norm, k_norm, pos, nullptr, 0, q, k, v, R, M, eps, stream);
+}
+
+// for gqa_tree.hip, which has checked its arguments: M <= 64, R a multiple of M
+__attribute__((visibility("hidden"))) int qt_internal_qkv_prep_tree(const void* qkv, const void* q_norm, const void* k_norm, const int32_t* pos,
+                                                                    const int32_t* parents, const void* rope_table, int table_positions, void* q, void* k,
+                                                                    void* v, long R, int M, float eps, hipStream_t stream) {
+    hipLaunchKernelGGL(attn_qkv_prep_kernel<true>, dim3((unsigned)((R + 3) / 4)), dim3(256), 0, stream, (const bf16_t*)qkv, (const bf16_t*)q_norm,
+                       (const bf16_t*)k_norm, pos, (bf16_t*)q, (bf16_t*)k, (bf16_t*)v, R, M, eps, (const float2*)rope_table, rope_table ? table_positions : 0,
+                       parents);
+    QT_CHECK_LAUNCH();
+    return QT_OK;
 }
 
 int qt_rope_table_build(void* table, int n_pos, hipStream_t stream) {

@@ -1,0 +1,501 @@
+// Attention of a tree of drafted tokens over a sequence's cache, 8 query heads on 2 KV heads, head dim 256, for gfx950.
+//
+// Row r = b * M + j is token j of sequence b.  It attends the pool keys below pos[b] and, among the M new keys of its sequence, those of its ancestors
+// and its own; new key j goes into the pool at pos[b] + j.  Up to 64 tokens share one pass over the cache (the chain form, gqa_decode.hip, takes four).
+//
+// Split over one flat space of 32-key tiles, as there: a segment (sequence, KV head) owns ceil(pos / 32) tiles of the pool and ceil(M / 32) of new keys, the
+// segments lie end to end, every workgroup takes the same number of consecutive tiles and writes an unnormalised partial result per segment that
+// it touches; a second kernel joins them.
+//   tiles  : HBM -> LDS directly, 4 buffers of K and V (16 KiB each), three tiles in flight.  A row is 32 pieces of 16 bytes; piece c of row r lies at place c ^ (r & 15),
+//            which spreads the 16 rows of a fragment over the banks
+//   scores : S^T[32 keys x 16 rows] = K . Q^T (16x16x32 bf16 MFMA); a row tile is four tokens x the four heads of the KV head; Q^T stays in registers
+//   P . V  : O^T[256 x 16 rows] += V^T . P^T, V^T through the transposing LDS load
+// Eight wavefronts: row tiles, and where there are few, key halves (KG) and halves of the 256 columns (CG) go to different ones.
+#include "tree.h"
+
+using namespace qt;
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int GQA = AH / AKV, QKV_W = AH * 2 * AD + 2 * AKV * AD;
+constexpr int KT = 32, ROW_BYTES = AD * 2, TILE_BYTES = KT * ROW_BYTES;        // keys a tile; bytes of its K (or V)
+constexpr int BUFS = 4, WAVES = 8, THREADS = 64 * WAVES;
+constexpr float SCALE_LOG2E = 0.0625f * 1.44269504088896f;                     // 256^-0.5 log2(e): the softmax works with powers of two
+constexpr float NEG = -3.0e38f;
+constexpr int MAX_SEG = 2048, MAX_GRID = 1024;
+
+__device__ __forceinline__ float max_over_groups(float x) {      // over the lanes n, n + 16, n + 32, n + 48
+    const unsigned xi = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(xi, xi, false, false);
+    const unsigned mi = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane16_swap(mi, mi, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+struct Plan {                           // how a launch cuts the flat tile space
+    int B, M, Lmax, n_slots, visit, min_tiles;
+};
+// tiles of a segment in the flat space: the pool's, the new keys', and `visit` empty positions for what a workgroup pays for a segment besides its tiles
+__device__ __forceinline__ int segment_tiles(const Plan& p, int slot, int p0) {
+    const bool ok = (unsigned)slot < (unsigned)p.n_slots && p0 >= 0 && p0 <= p.Lmax - p.M;
+    return ok ? (p0 + KT - 1) / KT + (p.M + KT - 1) / KT + p.visit : 0;
+}
+__device__ __forceinline__ int tiles_per_wg(int total, int nwg, int min_tiles) { return max(min_tiles, (total + nwg - 1) / nwg); }
+
+// a copy the compiler cannot see through: what is derived from it is computed again where it is used (the lane-dependent addresses of the tile loop would
+// live in about 50 registers across it)
+__device__ __forceinline__ int opaque(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+template <int N>
+__device__ __forceinline__ void wait_vmem() {                    // the direct-to-LDS loads are not the compiler's to count
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// RT row tiles a wavefront; NRG = 8 / (KG CG) groups of wavefronts with rows of their own
+template <int RT, int KG, int CG>
+__global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_new,
+                                                               const bf16_t* __restrict__ v_new, bf16_t* Kp, bf16_t* Vp,
+                                                               const int* __restrict__ slots, const int* __restrict__ pos,
+                                                               const int* __restrict__ parents, float* __restrict__ part_o,
+                                                               float* __restrict__ part_ml, int* __restrict__ seg_tab, const Plan plan) {
+    constexpr int NRG = WAVES / (KG * CG), ROWS = 16 * RT * NRG, KW = KT / KG, CB = 16 / CG;   // rows; keys of a tile and column blocks a wavefront takes
+    // P as two bf16 terms (off by 2^-17) while the launch is bound by the cache's bytes.  With two row tiles a wavefront the second product would cost a half
+    // more MFMA time: P is rounded once (2^-9 of each weight, the sum is taken of the rounded ones), less than the output's own rounding.
+    constexpr bool SPLIT = RT == 1;
+    __shared__ __align__(1024) unsigned char tile_s[BUFS * 2 * TILE_BYTES];
+    __shared__ int seg_start[MAX_SEG + 1];
+    __shared__ uint64_t seen_s[TREE_MAX];                        // bit i of entry j: token j sees new key i
+    __shared__ unsigned bad_s[2];
+    const int M = plan.M, nseg = plan.B * AKV;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int rg = w / (KG * CG), kg = w / CG % KG, cg = w % CG;
+
+    // ends of the segments in the flat space
+    {
+        __shared__ int wave_total[WAVES];
+        int carry = 0;
+        if (tid == 0) seg_start[0] = 0;
+        for (int base = 0; base < nseg; base += THREADS) {
+            const int sg = base + tid;
+            int v = sg < nseg ? segment_tiles(plan, slots[sg / AKV], pos[sg / AKV]) : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int u = __shfl_up(v, o);
+                if (lane >= o) v += u;
+            }
+            if (lane == 63) wave_total[w] = v;
+            __syncthreads();
+            int before = carry;
+            for (int i = 0; i < WAVES; i++) {
+                before += i < w ? wave_total[i] : 0;
+                carry += wave_total[i];
+            }
+            if (sg < nseg) seg_start[sg + 1] = before + v;
+            __syncthreads();
+        }
+        if (blockIdx.x == 0)
+            for (int i = tid; i <= nseg; i += THREADS) seg_tab[i] = seg_start[i];
+    }
+    const int total = __builtin_amdgcn_readfirstlane(seg_start[nseg]);
+    const int per = tiles_per_wg(total, gridDim.x, plan.min_tiles);
+    const int wt0 = blockIdx.x * per, wt1 = min(wt0 + per, total);
+    if (wt0 >= wt1) return;
+    int sg = 0;                                                  // the segment that holds position wt0
+    for (int hi = nseg; sg < hi;) {
+        const int mid = (sg + hi) >> 1;
+        if (__builtin_amdgcn_readfirstlane(seg_start[mid + 1]) <= wt0) sg = mid + 1; else hi = mid;
+    }
+    const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)tile_s);
+
+    for (; sg < nseg; sg++) {
+        const int begin = __builtin_amdgcn_readfirstlane(seg_start[sg]), end = __builtin_amdgcn_readfirstlane(seg_start[sg + 1]);
+        if (begin + plan.visit >= wt1) break;
+        if (end == begin || end <= wt0) continue;
+        const int b = sg / AKV, kvh = sg % AKV, slot = slots[b], p0 = pos[b];
+        const int pool_tiles = (p0 + KT - 1) / KT;
+        const int t0 = max(wt0 - begin - plan.visit, 0), t1 = min(wt1, end) - begin - plan.visit;      // tiles of the segment
+        const size_t pool_at = ((size_t)slot * AKV + kvh) * plan.Lmax * AD;
+        const bf16_t* const kn = k_new + ((size_t)b * M * AKV + kvh) * AD;
+        const bf16_t* const vn = v_new + ((size_t)b * M * AKV + kvh) * AD;
+
+        // rows w, w + 8, .. of pairs of a tile's rows: lane l brings place l & 31 of row 2 i + (l >> 5)
+        auto issue = [&](int t) {
+            const unsigned buf = lds0 + (unsigned)(t & (BUFS - 1)) * (2 * TILE_BYTES);
+            const int ln = opaque(lane);
+#pragma unroll
+            for (int i = 0; i < KT / 2 / WAVES; i++) {
+                const int r = 2 * (w + WAVES * i) + (ln >> 5), piece = (ln & 31) ^ (r & 15);
+                size_t at;
+                const bf16_t *ks, *vs;
+                if (t < pool_tiles) {                            // (a key past the end: the tile's first one instead, its weight is 0)
+                    const int key = t * KT + r < p0 ? t * KT + r : t * KT;
+                    at = pool_at + (size_t)key * AD;
+                    ks = Kp, vs = Vp;
+                } else {
+                    at = (size_t)min((t - pool_tiles) * KT + r, M - 1) * (AKV * AD);
+                    ks = kn, vs = vn;
+                }
+                const unsigned to = buf + (unsigned)(w + WAVES * i) * (2 * ROW_BYTES);
+                lds_dma16_from(reinterpret_cast<const char*>(ks + at) + 16 * piece, to);
+                lds_dma16_from(reinterpret_cast<const char*>(vs + at) + 16 * piece, to + TILE_BYTES);
+            }
+        };
+        constexpr int PER_TILE = KT / WAVES;                     // loads a wavefront issues per tile
+        // Q^T: lane (row n, group g) holds q[row n][32 kb + 8 g .. + 8] of each row tile
+        bf16x8 bq[RT][8];
+        {
+            const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const int tok = (rg * RT + t) * 4 + n / GQA;
+                const bf16_t* qr = q + ((size_t)(b * M + min(tok, M - 1)) * AH + kvh * GQA + n % GQA) * AD;
+#pragma unroll
+                for (int kb = 0; kb < 8; kb++) {
+                    u32x4 x = reinterpret_cast<const u32x4*>(qr)[kb * 4 + g];
+                    if (tok >= M) x = u32x4{0, 0, 0, 0};
+                    bq[t][kb] = __builtin_bit_cast(bf16x8, x);
+                }
+            }
+        }
+        if (w == 0) seen_s[lane] = tree_ancestors(tree_parent(parents + (size_t)b * M, lane, M), lane);
+        if (w == 0 && lane < 2) bad_s[lane] = 0;
+        __syncthreads();                                         // (also: the visit before is done with the tiles)
+        for (int i = 0; i < BUFS - 1; i++)
+            if (t0 + i < t1) issue(t0 + i);
+
+        f32x4 O[RT][CB];
+        float m_run[RT], l_run[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            m_run[t] = NEG, l_run[t] = 0.f;
+#pragma unroll
+            for (int j = 0; j < CB; j++) O[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int tile = t0; tile < t1; tile++) {
+            const int ahead = t1 - 1 - tile;                     // tiles that are in flight behind this one
+            if (ahead >= 2) wait_vmem<2 * PER_TILE>();
+            else if (ahead == 1) wait_vmem<PER_TILE>();
+            else wait_vmem<0>();
+            barrier();                                           // everyone's part of the tile has landed, and everyone is done with the buffer filled next
+            if (tile + BUFS - 1 < t1) issue(tile + BUFS - 1);
+            const unsigned char* const kt = tile_s + (tile & (BUFS - 1)) * (2 * TILE_BYTES);
+            unsigned char* const vt = tile_s + (tile & (BUFS - 1)) * (2 * TILE_BYTES) + TILE_BYTES;
+            const bool is_new = tile >= pool_tiles;
+            const int key0 = is_new ? (tile - pool_tiles) * KT : tile * KT, keys = is_new ? M : p0;
+            if (is_new) {
+                // A new value that is not finite must not reach rows that do not see it (0 times NaN): it becomes 0 here, and rows that do
+                // see its token become NaN at the end.  Rows past the last token become 0.
+#pragma unroll
+                for (int i = 0; i < TILE_BYTES / 16 / THREADS; i++) {
+                    const int at = 64 * w + opaque(lane) + THREADS * i, key = key0 + at / 32;
+                    u32x4 x = reinterpret_cast<u32x4*>(vt)[at];
+                    bool bad = false;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) bad |= (x[e] & 0x7f80) == 0x7f80 || (x[e] & 0x7f800000) == 0x7f800000;
+                    if (key >= M || bad) reinterpret_cast<u32x4*>(vt)[at] = u32x4{0, 0, 0, 0};
+                    if (key < M && bad) atomicOr(&bad_s[key >> 5], 1u << (key & 31));
+                }
+                __syncthreads();
+            }
+            const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+            f32x4 s[RT][KW / 16];
+#pragma unroll
+            for (int u = 0; u < KW / 16; u++) {
+                if (RT > 1) __builtin_amdgcn_sched_barrier(0);
+                const int row = kg * KW + 16 * u + n;            // A operand: lane (key n, group g) holds k[key][32 kb + 8 g .. + 8]
+                const unsigned at = row * ROW_BYTES + ((g ^ n) << 4);
+#pragma unroll
+                for (int t = 0; t < RT; t++) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kb = 0; kb < 8; kb++) {
+                    if (RT > 1 && kb == 4) __builtin_amdgcn_sched_barrier(0);
+                    const bf16x8 ka = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(kt + (at ^ (kb << 6))));
+#pragma unroll
+                    for (int t = 0; t < RT; t++) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, bq[t][kb], s[t][u], 0, 0, 0);
+                }
+            }
+            // online softmax: lane (row n, group g) holds keys 16 u + 4 g .. + 3
+            const bool masked = is_new || key0 + KT > keys;
+            u32x2 ph[RT][KW / 16], pl[SPLIT ? RT : 1][KW / 16];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                float mx = NEG;
+                const uint64_t seen = is_new ? seen_s[((rg * RT + t) * 4 + n / GQA) & 63] : 0;
+#pragma unroll
+                for (int u = 0; u < KW / 16; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float x = s[t][u][i] * SCALE_LOG2E;
+                        if (masked) {
+                            const int key = key0 + kg * KW + 16 * u + 4 * g + i;
+                            const bool on = is_new ? key < M && (seen >> (key & 63) & 1) : key < keys;
+                            x = on ? x : NEG;
+                        }
+                        s[t][u][i] = x;
+                        mx = fmaxf(mx, x);
+                    }
+                mx = max_over_groups(mx);
+                const float m_new = fmaxf(m_run[t], mx), corr = __builtin_amdgcn_exp2f(m_run[t] - m_new);
+                float sum = 0.f;
+#pragma unroll
+                for (int u = 0; u < KW / 16; u++) {
+                    float p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        p[i] = __builtin_amdgcn_exp2f(s[t][u][i] - m_new);
+                        if (masked && s[t][u][i] <= 0.5f * NEG) p[i] = 0.f;
+                        if constexpr (SPLIT) sum += p[i];
+                    }
+                    const u32x2 h = {pack2_bf(p[0], p[1]), pack2_bf(p[2], p[3])};
+                    ph[t][u] = h;
+                    if constexpr (SPLIT)
+                        pl[t][u] = u32x2{pack2_bf(p[0] - lo_bf(h[0]), p[1] - hi_bf(h[0])), pack2_bf(p[2] - lo_bf(h[1]), p[3] - hi_bf(h[1]))};
+                    else
+                        sum += (lo_bf(h[0]) + hi_bf(h[0])) + (lo_bf(h[1]) + hi_bf(h[1]));
+                }
+                l_run[t] = l_run[t] * corr + sum;                // this lane's share; summed over g at the end
+                m_run[t] = m_new;
+                if (__any(corr != 1.f)) {
+#pragma unroll
+                    for (int j = 0; j < CB; j++) O[t][j] *= corr;
+                }
+            }
+            // transposing load: lane (n, g) points at key 4 g + n / 4, columns 4 (n % 4) .. + 3 of the block, and receives keys 4 g .. + 3 of column n
+            const int vkey = kg * KW + 4 * g + (n >> 2);
+            const unsigned vat = vkey * ROW_BYTES + ((((n >> 1) & 1) ^ (vkey & 15)) << 4) + (n & 1) * 8;
+#pragma unroll
+            for (int j = 0; j < CB; j++) {
+                if (RT > 1 && j % 4 == 0) __builtin_amdgcn_sched_barrier(0);    // (at most four column blocks' fragments in registers at a time)
+                s16x4 a[KW / 16];
+#pragma unroll
+                for (int u = 0; u < KW / 16; u++)
+                    a[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4*)(vt + (vat ^ ((cg * CB + j) << 5)) + u * 16 * ROW_BYTES));
+                if constexpr (KW == 32) {
+                    const s16x4 a0 = a[0], a1 = a[1];
+                    const bf16x8 av = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        const u32x4 hp = {ph[t][0][0], ph[t][0][1], ph[t][1][0], ph[t][1][1]};
+                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, hp), O[t][j], 0, 0, 0);
+                        if constexpr (SPLIT) {
+                            const u32x4 lp = {pl[t][0][0], pl[t][0][1], pl[t][1][0], pl[t][1][1]};
+                            O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, lp), O[t][j], 0, 0, 0);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a[0], __builtin_bit_cast(s16x4, ph[t][0]), O[t][j], 0, 0, 0);
+                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a[0], __builtin_bit_cast(s16x4, pl[t][0]), O[t][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        // partial results of this visit, one per key group: [slot][ROWS][256] and (maximum, sum)
+        const uint64_t bad = (uint64_t)bad_s[1] << 32 | bad_s[0];
+        const size_t at = ((size_t)blockIdx.x + sg) * KG + kg;
+        {
+            const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const int row = (rg * RT + t) * 16 + n, tok = row / GQA;
+                const float l = sum_over_groups(l_run[t]);
+                if (tok < M) {
+                    float* po = part_o + (at * ROWS + row) * AD + cg * CB * 16 + 4 * g;
+#pragma unroll
+                    for (int j = 0; j < CB; j++) *reinterpret_cast<f32x4*>(po + 16 * j) = O[t][j];
+                    if (g == 0 && cg == 0) {
+                        part_ml[(at * ROWS + row) * 2] = m_run[t];
+                        part_ml[(at * ROWS + row) * 2 + 1] = seen_s[tok] & bad ? __builtin_nanf("") : l;
+                    }
+                }
+            }
+        }
+        // the new rows of this visit's tiles go into the pool (nobody reads it from pos on)
+        for (int i = 64 * w + opaque(lane) + max(t0 - pool_tiles, 0) * KT * 32, e = min((t1 - pool_tiles) * KT, M) * 32; i < e; i += THREADS) {
+            const int key = i / 32, c = i % 32;
+            const size_t to = (pool_at + (size_t)(p0 + key) * AD) / 8 + c, from = (size_t)key * (AKV * AD / 8) + c;
+            const u32x4 kx = reinterpret_cast<const u32x4*>(kn)[from], vx = reinterpret_cast<const u32x4*>(vn)[from];
+            reinterpret_cast<u32x4*>(Kp)[to] = kx;
+            reinterpret_cast<u32x4*>(Vp)[to] = vx;
+        }
+        __syncthreads();                                         // (the next visit clears what this one has collected)
+    }
+}
+
+// Joins the partial results: a wavefront per (sequence, token, head), a lane four columns.
+// GATE: out [R,2048] = BF(o * sigmoid_bf16(gate)), o rounded to bf16 before, as the separate kernels do
+template <bool GATE>
+__global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                                                              const int* __restrict__ seg_tab, bf16_t* __restrict__ out, const bf16_t* __restrict__ qkv,
+                                                              int nwg, int rows, int KG, const Plan plan) {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int id = blockIdx.x * 4 + w;
+    if (id >= plan.B * plan.M * AH) return;
+    const int head = id % AH, r = id / AH, b = r / plan.M, j = r % plan.M;
+    const int kvh = head / GQA, sg = b * AKV + kvh, row = j * GQA + head % GQA;
+    const int total = seg_tab[plan.B * AKV], ss = seg_tab[sg], se = seg_tab[sg + 1];
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float l = 1.f;
+    if (se > ss) {
+        const int per = tiles_per_wg(total, nwg, plan.min_tiles);
+        const int wg0 = (ss + plan.visit) / per, ns = ((se - 1) / per - wg0 + 1) * KG;
+        const size_t at = ((size_t)wg0 + sg) * KG;
+        const float* ml = part_ml + (at * rows + row) * 2;
+        const float* po = part_o + (at * rows + row) * AD + 4 * lane;
+        float mm = NEG;
+        for (int s = lane; s < ns; s += 64) mm = fmaxf(mm, ml[(size_t)s * rows * 2]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+        float lp = 0.f;
+        for (int s0 = 0; s0 < ns; s0 += 64) {
+            float f = 0.f;
+            if (s0 + lane < ns) {
+                const float2 x = *reinterpret_cast<const float2*>(ml + (size_t)(s0 + lane) * rows * 2);
+                f = __builtin_amdgcn_exp2f(x.x - mm);
+                lp += x.y * f;
+            }
+            const int here = min(64, ns - s0);
+            int s = 0;
+            for (; s + 4 <= here; s += 4) {
+                f32x4 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = *reinterpret_cast<const f32x4*>(po + (size_t)(s0 + s + i) * rows * AD);
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc += x[i] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s + i));
+            }
+            for (; s < here; s++) acc += *reinterpret_cast<const f32x4*>(po + (size_t)(s0 + s) * rows * AD) * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) lp += __shfl_xor(lp, o);
+        l = lp;
+    }
+    float o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = acc[i] / l;
+    if constexpr (GATE) {
+        const u32x2 gate = *reinterpret_cast<const u32x2*>(qkv + (size_t)r * QKV_W + head * 2 * AD + AD + 4 * lane);
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = se > ss ? BF(o[i]) * sigmoid_bf16(i & 1 ? hi_bf(gate[i >> 1]) : lo_bf(gate[i >> 1])) : 0.f;
+    }
+    *reinterpret_cast<u32x2*>(out + (size_t)id * AD + 4 * lane) = u32x2{pack2_bf(o[0], o[1]), pack2_bf(o[2], o[3])};
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int grid_size() {
+    const int cus = qt::cu_count();
+    return cus < MAX_GRID ? cus : MAX_GRID;
+}
+// rows of a partial result, and key groups
+inline void shape(int M, int& rows, int& kg) {
+    rows = M <= 8 ? 32 : M <= 16 ? 64 : M <= 32 ? 128 : 256;
+    kg = M <= 16 ? 2 : 1;
+}
+constexpr long SEG_TAB_BYTES = ((MAX_SEG + 1) * 4 + 15) / 16 * 16;
+
+int launch(const void* q, const void* k, const void* v, void* Kp, void* Vp, const int32_t* slots, const int32_t* pos, const int32_t* parents, void* out,
+           const void* gate_rows, void* workspace, int B, int M, int Lmax, int n_slots, hipStream_t stream) {
+    int rows, kg;
+    shape(M, rows, kg);
+    const int nwg = grid_size();
+    const size_t cap = ((size_t)nwg + (size_t)B * AKV) * kg;
+    float* const part_o = (float*)workspace;
+    float* const part_ml = part_o + cap * rows * AD;
+    int* const seg_tab = reinterpret_cast<int*>(part_ml + cap * rows * 2);
+    const Plan plan = {B, M, Lmax, n_slots, 2 + rows / 64, 2};
+#define QT_TREE_ATTN(RT, KG, CG)                                                                                                                       \
+    hipLaunchKernelGGL((attn_tree_kernel<RT, KG, CG>), dim3((unsigned)nwg), dim3(THREADS), 0, stream, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, \
+                       (bf16_t*)Kp, (bf16_t*)Vp, slots, pos, parents, part_o, part_ml, seg_tab, plan)
+    if (M <= 8) QT_TREE_ATTN(1, 2, 2);
+    else if (M <= 16) QT_TREE_ATTN(1, 2, 1);
+    else if (M <= 32) QT_TREE_ATTN(1, 1, 1);
+    else QT_TREE_ATTN(2, 1, 1);
+#undef QT_TREE_ATTN
+    QT_CHECK_LAUNCH();
+    const dim3 grid((unsigned)((B * M * AH + 3) / 4));
+    if (gate_rows)
+        hipLaunchKernelGGL(attn_tree_merge_kernel<true>, grid, dim3(256), 0, stream, part_o, part_ml, seg_tab, (bf16_t*)out, (const bf16_t*)gate_rows, nwg, rows, kg, plan);
+    else
+        hipLaunchKernelGGL(attn_tree_merge_kernel<false>, grid, dim3(256), 0, stream, part_o, part_ml, seg_tab, (bf16_t*)out, (const bf16_t*)nullptr, nwg, rows, kg, plan);
+    QT_CHECK_LAUNCH();
+    return QT_OK;
+}
+
+int check(int B, int M, int Lmax, int n_slots) {
+    if (B < 0 || Lmax < 1 || n_slots < 1) return QT_ERR_DIM;
+    if (M < 1 || M > TREE_MAX || B > MAX_SEG / AKV) return QT_ERR_UNSUPPORTED;
+    return QT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+// (attn_glue.hip) the q / k norm, rotary embedding and split of qkv rows whose positions follow from a tree
+int qt_internal_qkv_prep_tree(const void* qkv, const void* q_norm, const void* k_norm, const int32_t* pos, const int32_t* parents, const void* rope_table,
+                              int table_positions, void* q, void* k, void* v, long R, int M, float eps, hipStream_t stream) __attribute__((visibility("hidden")));
+
+static long partial_bytes(int B, int M) {
+    int rows, kg;
+    shape(M, rows, kg);
+    return ((long)grid_size() + (long)B * AKV) * kg * rows * (AD + 2) * 4 + SEG_TAB_BYTES;
+}
+
+long qt_gqa_tree_workspace_bytes(int B, int M) {
+    if (B < 0 || B > MAX_SEG / AKV || M < 1 || M > TREE_MAX) return -1;
+    return partial_bytes(B, M);
+}
+long qt_gqa_tree_layer_workspace_bytes(int B, int M) {
+    const long n = qt_gqa_tree_workspace_bytes(B, M);
+    return n < 0 ? n : n + (long)B * M * (AH + 2 * AKV) * AD * 2;
+}
+
+int qt_gqa_tree_attn(const void* q, const void* k_new, const void* v_new, void* Kp, void* Vp, const int32_t* slots, const int32_t* pos,
+                     const int32_t* parents, void* out, void* workspace, long workspace_bytes, int B, int M, int Lmax, int n_slots, hipStream_t stream) {
+    if (const int rc = check(B, M, Lmax, n_slots)) return rc;
+    if (B == 0) return QT_OK;
+    if (!q || !k_new || !v_new || !Kp || !Vp || !slots || !pos || !parents || !out || !workspace) return QT_ERR_NULL;
+    for (const void* p : {q, k_new, v_new, (const void*)Kp, (const void*)Vp, (const void*)out, (const void*)workspace})
+        if (!aligned16(p)) return QT_ERR_ALIGN;
+    if (workspace_bytes < qt_gqa_tree_workspace_bytes(B, M)) return QT_ERR_WORKSPACE;
+    return launch(q, k_new, v_new, Kp, Vp, slots, pos, parents, out, nullptr, workspace, B, M, Lmax, n_slots, stream);
+}
+
+int qt_gqa_tree_layer(const void* qkv, const void* q_norm, const void* k_norm, const void* rope_table, int table_positions, void* Kp, void* Vp,
+                      const int32_t* slots, const int32_t* pos, const int32_t* parents, void* out, void* workspace, long workspace_bytes, int B, int M,
+                      int Lmax, int n_slots, float eps, hipStream_t stream) {
+    if (const int rc = check(B, M, Lmax, n_slots)) return rc;
+    if (table_positions < 0 || (table_positions > 0 && !rope_table)) return QT_ERR_DIM;
+    if (B == 0) return QT_OK;
+    if (!qkv || !q_norm || !k_norm || !Kp || !Vp || !slots || !pos || !parents || !out || !workspace) return QT_ERR_NULL;
+    for (const void* p : {qkv, q_norm, k_norm, rope_table, (const void*)Kp, (const void*)Vp, (const void*)out, (const void*)workspace})
+        if (!aligned16(p)) return QT_ERR_ALIGN;
+    if (workspace_bytes < qt_gqa_tree_layer_workspace_bytes(B, M)) return QT_ERR_WORKSPACE;
+    bf16_t* const q = reinterpret_cast<bf16_t*>((char*)workspace + partial_bytes(B, M));
+    bf16_t* const k = q + (size_t)B * M * AH * AD;
+    bf16_t* const v = k + (size_t)B * M * AKV * AD;
+    if (const int rc = qt_internal_qkv_prep_tree(qkv, q_norm, k_norm, pos, parents, rope_table, table_positions, q, k, v, (long)B * M, M, eps, stream)) return rc;
+    return launch(q, k, v, Kp, Vp, slots, pos, parents, out, qkv, workspace, B, M, Lmax, n_slots, stream);
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -208,7 +209,7 @@ struct Busy {
         if (m) m->unlock();
     }
 };
-enum Purpose { ATTN_B, PREFILL_ATTENTION };
+enum Purpose { ATTN_B, PREFILL_ATTENTION, TREE_ATTENTION, BEAM_SELECT };
 Scratch workspace(int purpose, const Tensor& like, long bytes, long first) {
     if (capturing()) return {unlocked([&] { return empty({bytes}, U8, like); }), nullptr};
     struct Kept {
@@ -910,6 +911,200 @@ PyObject* cache_restore(PyObject* const* a) {
     return PyTuple_Pack(3, kv.o, cs.o, ss.o);
 }
 
+// ---- several branches: drafted trees and beams ------------------------------------------------------------------------------
+// These run on the device of their tensors (all on one), whichever is current, and on its current stream.
+struct OnDevice {
+    c10::DeviceGuard guard;
+    const at::Device device;
+    explicit OnDevice(const Tensor& t) : guard(t.device()), device(t.device()) {}
+    void operator()(const Tensor& t, const char* name) const {
+        if (t.device() != device) value_error(std::string(name) + ": on " + t.device().str() + ", expected " + device.str());
+    }
+};
+// parents [B, M] int32 for B * M = R rows
+int64_t tree_tokens(const Tensor& parents, int64_t R, const char* who) {
+    const int64_t B = parents.size(0), M = parents.size(1);
+    if (M < 1 || M > 64) value_error(std::string(who) + ": " + std::to_string(M) + " tokens a tree, 1..64 are possible");
+    if (B * M != R) value_error(std::string(who) + ": " + std::to_string(R) + " rows for trees " + shape_text(parents.sizes().vec()));
+    return M;
+}
+
+// deltanet_bt(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents)
+PyObject* deltanet_bt(PyObject* const* a) {
+    const Tensor& proj = dev(a[0], BF16, "proj", {ANY, PW});
+    const Tensor& parents = dev(a[8], I32, "parents", {ANY, ANY});
+    const int64_t M = tree_tokens(parents, proj.size(0), "deltanet_bt"), B = parents.size(0);
+    const Tensor& ssm = dev(a[5], F32, "ssm_pool", {ANY, HV, DV, DK});
+    const int64_t n_slots = ssm.size(0);
+    const Tensor& conv = dev(a[1], BF16, "conv_pool", {n_slots * 2, 3, CD});
+    const Tensor &slots = dev(a[6], I32, "slots", {B}), &pos = dev(a[7], I32, "pos", {B}), &w = flat_conv_w(a[2]);
+    const OnDevice on(proj);
+    const Tensor A = f32(a[3], "A_log", HV), dtb = f32(a[4], "dt_bias", HV);
+    on(conv, "conv_pool"), on(w, "conv_w"), on(A, "A_log"), on(dtb, "dt_bias"), on(ssm, "ssm_pool"), on(slots, "slots"), on(pos, "pos"), on(parents, "parents");
+    return wrap(unlocked([&] {
+        Tensor y = empty({B * M, HV * DV}, BF16, proj);
+        check(qt_gdn_tree_step(proj.data_ptr(), conv.data_ptr(), w.data_ptr(), A.data_ptr<float>(), dtb.data_ptr<float>(), ssm.data_ptr<float>(),
+                               slots.data_ptr<int>(), pos.data_ptr<int>(), parents.data_ptr<int>(), y.data_ptr(), dim32(B), dim32(M), dim32(n_slots), stream()),
+              "qt_gdn_tree_step");
+        return y;
+    }));
+}
+
+// attn_bt(q, k, v, Kp, Vp, slots, pos, parents)
+PyObject* attn_bt(PyObject* const* a) {
+    const Tensor& q = dev(a[0], BF16, "q", {ANY, 8, 256});
+    const int64_t R = q.size(0);
+    const Tensor &k = dev(a[1], BF16, "k", {R, 2, 256}), &v = dev(a[2], BF16, "v", {R, 2, 256}), &parents = dev(a[7], I32, "parents", {ANY, ANY});
+    const int64_t M = tree_tokens(parents, R, "attn_bt"), B = parents.size(0);
+    const Pool p = kv_pool(a[3], a[4], a[5], a[6], B);
+    const OnDevice on(q);
+    on(k, "k"), on(v, "v"), on(p.K, "Kp"), on(p.V, "Vp"), on(p.slots, "slots"), on(p.pos, "pos"), on(parents, "parents");
+    const long bytes = qt_gqa_tree_workspace_bytes(dim32(B), dim32(M));
+    if (bytes < 0) value_error("attn_bt: " + std::to_string(B) + " sequences, 1024 are possible");
+    const Scratch ws = workspace(TREE_ATTENTION, q, bytes, 0);
+    return wrap(unlocked([&] {
+        Tensor o = empty({R, 8, 256}, BF16, q);
+        const Busy busy(ws.busy);
+        check(qt_gqa_tree_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), p.K.data_ptr(), p.V.data_ptr(), p.slots.data_ptr<int>(), p.pos.data_ptr<int>(),
+                               parents.data_ptr<int>(), o.data_ptr(), ws.buf.data_ptr(), ws.buf.numel(), dim32(B), dim32(M), dim32(p.Lmax), dim32(p.n_slots),
+                               stream()), "qt_gqa_tree_attn");
+        return o;
+    }));
+}
+
+// attn_layer_bt(qkv, q_norm, k_norm, Kp, Vp, slots, pos, parents, eps)
+PyObject* attn_layer_bt(PyObject* const* a) {
+    const Tensor& qkv = dev(a[0], BF16, "qkv", {ANY, QKV_W});
+    const int64_t R = qkv.size(0);
+    const Tensor &qn = dev(a[1], BF16, "q_norm", {256}), &kn = dev(a[2], BF16, "k_norm", {256}), &parents = dev(a[7], I32, "parents", {ANY, ANY});
+    const int64_t M = tree_tokens(parents, R, "attn_layer_bt"), B = parents.size(0);
+    const Pool p = kv_pool(a[3], a[4], a[5], a[6], B);
+    const float eps = real(a[8]);
+    const OnDevice on(qkv);
+    on(qn, "q_norm"), on(kn, "k_norm"), on(p.K, "Kp"), on(p.V, "Vp"), on(p.slots, "slots"), on(p.pos, "pos"), on(parents, "parents");
+    const long bytes = qt_gqa_tree_layer_workspace_bytes(dim32(B), dim32(M));
+    if (bytes < 0) value_error("attn_layer_bt: " + std::to_string(B) + " sequences, 1024 are possible");
+    const Scratch ws = workspace(TREE_ATTENTION, qkv, bytes, 0);
+    const Tensor table = rope_table(qkv, p.Lmax);
+    return wrap(unlocked([&] {
+        Tensor out = empty({R, 2048}, BF16, qkv);
+        const Busy busy(ws.busy);
+        check(qt_gqa_tree_layer(qkv.data_ptr(), qn.data_ptr(), kn.data_ptr(), table.data_ptr(), dim32(table.size(0)), p.K.data_ptr(), p.V.data_ptr(),
+                                p.slots.data_ptr<int>(), p.pos.data_ptr<int>(), parents.data_ptr<int>(), out.data_ptr(), ws.buf.data_ptr(), ws.buf.numel(),
+                                dim32(B), dim32(M), dim32(p.Lmax), dim32(p.n_slots), eps, stream()), "qt_gqa_tree_layer");
+        return out;
+    }));
+}
+
+// The layers of a stack's pools (lists of tensors, all of one shape), checked, as tables of pointers
+struct PoolList {
+    std::vector<float*> ssm;
+    std::vector<void*> conv, kv;
+    int64_t n_slots = -1, Lmax = 0;
+    PoolList(PyObject* convs, PyObject* ssms, PyObject* Ks, PyObject* Vs, const OnDevice& on) {
+        const Items pc(convs), ps(ssms), pk(Ks), pv(Vs);
+        if (pc.size() != ps.size()) value_error("pools: as many conv as ssm layers expected");
+        if (pk.size() != pv.size()) value_error("pools: as many K as V layers expected");
+        for (Py_ssize_t i = 0; i < ps.size(); i++) {
+            const Tensor& s = dev(ps[i], F32, "ssm", {n_slots, HV, DV, DK});
+            n_slots = s.size(0);
+            const Tensor& c = dev(pc[i], BF16, "conv", {n_slots * 2, 3, CD});
+            on(s, "ssm"), on(c, "conv");
+            ssm.push_back(s.data_ptr<float>());
+            conv.push_back(c.data_ptr());
+        }
+        for (Py_ssize_t i = 0; i < 2 * pk.size(); i++) {
+            const Tensor& t = dev(i & 1 ? pv[i / 2] : pk[i / 2], BF16, i & 1 ? "V" : "K", {n_slots, 2, i ? Lmax : ANY, 256});
+            n_slots = t.size(0), Lmax = t.size(2);
+            on(t, i & 1 ? "V" : "K");
+            kv.push_back(t.data_ptr());
+        }
+        if (n_slots < 0) value_error("pools: no layers");
+    }
+};
+
+// tree_commit(conv pools, ssm pools, K pools, V pools, projs, conv_ws, A_logs, dt_biases, slots, pos, path, count, M or None)
+PyObject* tree_commit(PyObject* const* a) {
+    const Tensor& path = dev(a[10], I32, "path", {ANY, ANY});
+    const int64_t B = path.size(0), D = path.size(1);
+    if (D < 1 || D > 64) value_error("commit: paths of up to " + std::to_string(D) + " tokens, 1..64 are possible");
+    const Tensor &count = dev(a[11], I32, "count", {B}), &slots = dev(a[8], I32, "slots", {B}), &pos = dev(a[9], I32, "pos", {B});
+    const OnDevice on(path);
+    on(count, "count"), on(slots, "slots"), on(pos, "pos");
+    const PoolList p(a[0], a[1], a[2], a[3], on);
+    const Items projs(a[4]), cws(a[5]), As(a[6]), dts(a[7]);
+    const size_t n = p.ssm.size();
+    for (const Items* l : {&projs, &cws, &As, &dts})
+        if ((size_t)l->size() != n) value_error("commit: projs, conv_ws, A_logs and dt_biases need one entry for each of the " + std::to_string(n) + " recurrent layers");
+    int64_t M = a[12] == Py_None ? 0 : integer(a[12]);
+    std::vector<const void*> proj, cw;
+    std::vector<const float*> A, dtb;
+    std::vector<Tensor> held;                                    // (what had to be converted)
+    for (size_t i = 0; i < n; i++) {
+        const Tensor& t = dev(projs[i], BF16, "proj", {ANY, PW});
+        if (M == 0 && B > 0) M = t.size(0) / B;
+        if (t.size(0) != B * M) value_error("commit: proj: expected " + std::to_string(B * M) + " rows (" + std::to_string(B) + " trees), got " + std::to_string(t.size(0)));
+        const Tensor& w = flat_conv_w(cws[i]);
+        const Tensor Ai = f32(As[i], "A_log", HV), di = f32(dts[i], "dt_bias", HV);
+        on(t, "proj"), on(w, "conv_w"), on(Ai, "A_log"), on(di, "dt_bias");
+        held.push_back(Ai), held.push_back(di);
+        proj.push_back(t.data_ptr()), cw.push_back(w.data_ptr()), A.push_back(Ai.data_ptr<float>()), dtb.push_back(di.data_ptr<float>());
+    }
+    if (B == 0) Py_RETURN_NONE;
+    if (M < 1 || M > 64) value_error("commit: trees of " + std::to_string(M) + " tokens, 1..64 are possible");
+    unlocked([&] {
+        check(qt_tree_commit(proj.data(), p.conv.data(), cw.data(), A.data(), dtb.data(), p.ssm.data(), (int)n, p.kv.data(), (int)p.kv.size(), slots.data_ptr<int>(),
+                             pos.data_ptr<int>(), path.data_ptr<int>(), count.data_ptr<int>(), dim32(B), dim32(M), dim32(D), dim32(p.n_slots), dim32(p.Lmax), stream()),
+              "qt_tree_commit");
+    });
+    Py_RETURN_NONE;
+}
+
+// beam_select(logits, scores, n) -> scores, parents, tokens
+PyObject* beam_select(PyObject* const* a) {
+    const Tensor& x = gpu_tensor(a[0], "logits");
+    const ScalarType t = x.scalar_type();
+    if (t != BF16 && t != F16 && t != F32) type_error(std::string("logits: expected torch.bfloat16, torch.float16 or torch.float32, got ") + dtype_text(t));
+    check_shape(x, "logits", {ANY, ANY, ANY});
+    const int64_t G = x.size(0), W = x.size(1), V = x.size(2), n = integer(a[2]);
+    if (W < 1 || W > 64) value_error("select: " + std::to_string(W) + " beams, 1..64 are possible");
+    if (n < 1 || n > 64) value_error("select: n = " + std::to_string(n) + ", 1..64 are possible");
+    if (V < 1 || V > INT_MAX) value_error("select: an empty or too large vocabulary");
+    if (V > 1 && x.stride(2) != 1) value_error("logits: the vocabulary must be contiguous");
+    if (G * W > 65535) value_error("select: " + std::to_string(G) + " x " + std::to_string(W) + " beams, 65535 are possible");
+    const Tensor& scores = dev(a[1], F32, "scores", {G, W});
+    const OnDevice on(x);
+    on(scores, "scores");
+    const long bytes = qt_beam_select_workspace_bytes(G, dim32(W), dim32(V), dim32(n), (int)x.element_size());
+    if (bytes < 0) value_error("select: bad sizes");
+    const Scratch ws = workspace(BEAM_SELECT, x, std::max(bytes, 16L), 1 << 20);
+    Tensor s, w, tok;
+    unlocked([&] {
+        s = empty({G, n}, F32, x), w = empty({G, n}, I32, x), tok = empty({G, n}, I32, x);
+        if (G == 0) return;
+        const Busy busy(ws.busy);
+        check(qt_beam_select(x.data_ptr(), t == BF16 ? 0 : t == F16 ? 1 : 2, x.stride(0), x.stride(1), scores.data_ptr<float>(), s.data_ptr<float>(), w.data_ptr<int>(),
+                             tok.data_ptr<int>(), ws.buf.data_ptr(), ws.buf.numel(), dim32(G), dim32(W), dim32(V), dim32(n), stream()), "qt_beam_select");
+    });
+    return wrap({s, w, tok});
+}
+
+// beam_reorder(conv pools, ssm pools, K pools, V pools, slots, parents, start, pos)
+PyObject* beam_reorder(PyObject* const* a) {
+    const Tensor& slots = dev(a[4], I32, "slots", {ANY, ANY});
+    const int64_t G = slots.size(0), W = slots.size(1);
+    if (W < 1 || W > 32) value_error("reorder: " + std::to_string(W) + " beams, 1..32 are possible");
+    const Tensor &parents = dev(a[5], I32, "parents", {G, W}), &start = dev(a[6], I32, "start", {G}), &pos = dev(a[7], I32, "pos", {G});
+    const OnDevice on(slots);
+    on(parents, "parents"), on(start, "start"), on(pos, "pos");
+    const PoolList p(a[0], a[1], a[2], a[3], on);
+    unlocked([&] {
+        check(qt_beam_reorder(p.ssm.data(), p.conv.data(), (int)p.ssm.size(), p.kv.data(), (int)p.kv.size(), slots.data_ptr<int>(), parents.data_ptr<int>(),
+                              start.data_ptr<int>(), pos.data_ptr<int>(), dim32(G), dim32(W), dim32(p.n_slots), dim32(p.Lmax), stream()), "qt_beam_reorder");
+    });
+    Py_RETURN_NONE;
+}
+
 // ---- the module -----------------------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -943,6 +1138,8 @@ PyMethodDef methods[] = {
     QT_FN("gdn_core", gdn_core, 7),
     QT_FN("set_hooks", set_hooks, 3),     QT_FN("blit_batch", blit_batch, 2),     QT_FN("pools_load", pools_load, 12),
     QT_FN("cache_restore", cache_restore, 5),
+    QT_FN("deltanet_bt", deltanet_bt, 9), QT_FN("attn_bt", attn_bt, 8),           QT_FN("attn_layer_bt", attn_layer_bt, 9),
+    QT_FN("tree_commit", tree_commit, 13), QT_FN("beam_select", beam_select, 3),  QT_FN("beam_reorder", beam_reorder, 8),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_qt_host", "argument checks, allocation and launch of the operators", -1, methods};
 
