@@ -4,6 +4,7 @@
 // W V candidates, equal ones by the lower index w V + t.  The logits are read once: a launch over slices of the vocabulary keeps, per slice,
 // its n largest logits and its part (maximum, sum) of l_w; a second launch joins the slices of a sequence's beams.
 #include "qt_common.h"
+#include <algorithm>
 
 using namespace qt;
 
@@ -15,6 +16,7 @@ typedef _Float16 f16;
 constexpr int SELECT_MAX = 64;          // beams of a sequence, and candidates to select
 constexpr int WAVE_CAP = 256;           // candidates a wavefront holds before it keeps the best n of them
 constexpr int NO_INDEX = 0x7fffffff;
+constexpr float LOG2E = 1.44269504088896f;
 
 __device__ __forceinline__ float as_float(bf16_t v) { return bf2f(v); }
 __device__ __forceinline__ float as_float(f16 v) { return (float)v; }
@@ -31,15 +33,38 @@ __device__ __forceinline__ unsigned order_bits(float f) {
 }
 __device__ __forceinline__ float from_order_bits(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// the largest value v whose low 16 order bits are zero such that n of the wavefront's lanes hold at least v; n <= 64
-__device__ __forceinline__ unsigned wave_nth_bits(unsigned key, int n) {
+// over the wavefront, every lane gets it: four steps within a row of 16 lanes, two exchanges of rows (a shuffle goes through the LDS pipeline)
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_mov<0xB1>(v));
+    v = fmaxf(v, dpp_mov<0x4E>(v));
+    v = fmaxf(v, dpp_mov<0x141>(v));
+    v = fmaxf(v, dpp_mov<0x140>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = row16_sum(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// A lower bound of the wavefront's n-th largest value, n <= 64: its highest order bits, two at a time, until just n are left or 16 bits are known
+__device__ __forceinline__ float wave_nth(float x, int n) {
+    const unsigned key = order_bits(x);
     unsigned v = 0;
-#pragma unroll
-    for (int bit = 31; bit >= 16; bit--) {
-        const unsigned t = v | 1u << bit;
-        if (__popcll(__ballot(key >= t)) >= n) v = t;
+    int c = 64;
+#pragma unroll 1
+    for (int bit = 30; bit >= 16 && c > n; bit -= 2) {
+        const int c1 = __popcll(__ballot(key >= (v | 1u << bit))), c2 = __popcll(__ballot(key >= (v | 2u << bit))), c3 = __popcll(__ballot(key >= (v | 3u << bit)));
+        if (c3 >= n) v |= 3u << bit, c = c3;
+        else if (c2 >= n) v |= 2u << bit, c = c2;
+        else if (c1 >= n) v |= 1u << bit, c = c1;
     }
-    return v;
+    const float f = from_order_bits(v);
+    return f == f ? f : -INFINITY;
 }
 
 struct Cand {                           // a logit and its place in the vocabulary
@@ -75,10 +100,10 @@ __device__ __forceinline__ int wave_keep_best(Cand* list, int count, int n, int 
 // the 16 bytes of logits number `piece` of a row; what lies behind the row reads as -inf.  The pieces count from the row's first logit wherever it lies in memory (the
 // hardware loads 16 bytes from any element), so that equal rows have equal sums, bit for bit.
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, long piece, int V, float (&x)[16 / sizeof(T)]) {
+__device__ __forceinline__ void load_piece(const T* row, unsigned piece, unsigned V, float (&x)[16 / sizeof(T)]) {
     constexpr int N = 16 / sizeof(T);
     typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
-    const long t0 = piece * N;
+    const unsigned t0 = piece * N;                               // (V < 2^31: no sum passes 2^32)
     if (t0 + N <= V) {
         union {
             u32x4 v;
@@ -93,96 +118,111 @@ __device__ __forceinline__ void load_piece(const T* row, long piece, int V, floa
     }
 }
 
-// Workgroup (slice p, row r) of four wavefronts, each on a part of its own of the slice, in tiles of 64 lanes x 4 pieces of 16 bytes.
-// A wavefront keeps a list of candidates in LDS.  What enters has to be at least as large as a threshold: after the first tile the n-th largest of
-// the lanes' maxima (n different logits are no smaller), later the n-th best of the list, taken whenever it has filled.  So almost every
-// logit costs a comparison, its exponential, and no more.
+// Workgroup (slice p, beam, sequence) of four wavefronts, each on `per_wave` tiles of its own of the beam's row: 64 lanes x 4 pieces of 16 bytes.
+// What becomes a candidate has to be at least as large as a threshold.  At first that is the largest of the wavefronts' n-th largest lane maxima of their first
+// tiles (n different logits are no smaller): of a random row about n candidates a workgroup are left, and almost every logit costs its
+// exponential, a comparison and no more.  A wavefront collects its candidates in LDS; when the list has filled (rising or equal logits), it keeps the best
+// n and raises its threshold.
 template <typename T>
-__global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ logits, long stride_g, long stride_w, int W, int V, int n, int slices,
-                                                          Cand* __restrict__ best, float2* __restrict__ part) {
+__global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ logits, long stride_g, long stride_w, unsigned V, int n,
+                                                          unsigned tiles, unsigned per_wave, Cand* __restrict__ best, float2* __restrict__ part) {
     constexpr int N = 16 / sizeof(T), PIECES = 4, TILE = 64 * PIECES;         // pieces a tile
-    __shared__ Cand list_s[4][WAVE_CAP];
+    __shared__ Cand list_s[4][WAVE_CAP], flat_s[256];
     __shared__ int count_s[4];
+    __shared__ float thr_s[4];
     __shared__ float2 ml_s[4];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int p = blockIdx.x, r = blockIdx.y;
-    const T* const row = logits + (long)(r / W) * stride_g + (long)(r % W) * stride_w;
-    const long pieces = ((long)V + N - 1) / N, tiles = (pieces + TILE - 1) / TILE;
-    // tiles of the row dealt out evenly to 4 * slices wavefronts
-    const long parts = 4l * slices, me = 4l * p + w;
-    const long first = tiles * me / parts, last = tiles * (me + 1) / parts;
+    const unsigned p = blockIdx.x, slices = gridDim.x, r = blockIdx.z * gridDim.y + blockIdx.y;
+    const T* const row = logits + (long)blockIdx.z * stride_g + (long)blockIdx.y * stride_w;
+    const unsigned first = min((4 * p + w) * per_wave, tiles), last = min(first + per_wave, tiles);
     Cand* const list = list_s[w];
     int count = 0;
     float m = -INFINITY, l = 0.f;
     float thr = -INFINITY;                                       // candidates are (x, t) at or before (thr, thr_t)
     int thr_t = NO_INDEX;
-    for (long tile = first; tile < last; tile++) {
-        float x[PIECES][N];
+    if (first == last && lane == 0) thr_s[w] = -INFINITY;
+    for (unsigned tile = first; tile < last || tile == first; tile++) {
+        const bool real = tile < last;
+        float x[PIECES][N], pm[PIECES];                          // and the pieces' maxima
+        if (real) {
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) load_piece(row, tile * TILE + 64 * i + lane, V, x[i]);
-        float top = -INFINITY;
+            for (int i = 0; i < PIECES; i++) load_piece(row, tile * TILE + 64 * i + lane, V, x[i]);
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                pm[i] = fmaxf(x[i][0], x[i][1]);
+#pragma unroll
+                for (int e = 2; e < N; e += 2) pm[i] = fmaxf(fmaxf(pm[i], x[i][e]), x[i][e + 1]);
+            }
+            const float top = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
+            if (tile == first) {
+                const float t = wave_nth(top, n);
+                if (lane == 0) thr_s[w] = t;
+            }
+            const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < PIECES; i++)
+#pragma unroll
+                for (int e = 0; e < N; e++) sum[e & 3] += __builtin_amdgcn_exp2f((x[i][e] - ref) * LOG2E);        // (x log2 e - ref log2 e would lose bits, or overflow)
+            l = l * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));      // (m = -inf: l is 0, or NaN already)
+            m = m_new;
+        }
+        if (tile == first) {                                     // (every wavefront comes by once)
+            __syncthreads();
+            thr = fmaxf(fmaxf(thr_s[0], thr_s[1]), fmaxf(thr_s[2], thr_s[3]));
+        }
+        if (!real) break;
+        unsigned hits = 0;                                       // bit i * N + e
+        const float low = fmaxf(thr, -3.402823466e38f);          // (-inf is no candidate)
 #pragma unroll
         for (int i = 0; i < PIECES; i++)
+            if (__any(pm[i] >= low)) {
 #pragma unroll
-            for (int e = 0; e < N; e++) top = fmaxf(top, x[i][e]);
-        const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < PIECES; i++)
-#pragma unroll
-            for (int e = 0; e < N; e++) sum += __expf(x[i][e] - ref);
-        l = l * __expf(m - ref) + sum;                           // (m = -inf: l is 0, or NaN already)
-        m = m_new;
-        if (tile == first) thr = from_order_bits(wave_nth_bits(order_bits(top), n));
-        if (!(thr == thr)) thr = -INFINITY;
-#pragma unroll 1
-        for (int i = 0; i < PIECES; i++) {
-            bool any = false;
-            float xi[N];
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                xi[e] = i == 0 ? x[0][e] : i == 1 ? x[1][e] : i == 2 ? x[2][e] : x[3][e];
-                any |= xi[e] >= thr;
+                for (int e = 0; e < N; e++) hits |= x[i][e] >= low ? 1u << (i * N + e) : 0u;
             }
-            if (!__any(any)) continue;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const int t = (int)((tile * TILE + 64 * i + lane) * N + e);
-                const bool in = xi[e] > -INFINITY && (xi[e] > thr || (xi[e] == thr && t <= thr_t));
-                const uint64_t who = __ballot(in);
-                if (!who) continue;
-                if (count + 64 > WAVE_CAP) {
-                    count = wave_keep_best(list, count, n, lane);
-                    if (count == n) thr = list[n - 1].x, thr_t = list[n - 1].t;
-                }
-                if (in) list[count + __popcll(who & ((1ull << lane) - 1))] = Cand{xi[e], t};
-                count += __popcll(who);
+        while (__any(hits)) {                                    // each lane's next one; read again, which costs less than to find it among the registers
+            const unsigned k = __builtin_ctz(hits | 1u << 31);
+            const int t = (int)((tile * TILE + 64 * (k / N) + lane) * N + k % N);
+            const float v = hits ? as_float(row[t]) : -INFINITY;
+            const bool in = hits && (v > thr || (v == thr && t <= thr_t));
+            hits &= hits - 1;
+            const uint64_t who = __ballot(in);
+            if (count + 64 > WAVE_CAP) {
+                count = wave_keep_best(list, count, n, lane);
+                if (count == n) thr = list[n - 1].x, thr_t = list[n - 1].t;
             }
+            if (in) list[count + __popcll(who & ((1ull << lane) - 1))] = Cand{v, t};
+            count += __popcll(who);
         }
     }
-    count = wave_keep_best(list, count, n, lane);
     // the wavefront's part of l_w
     {
-        float mm = m;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
-        const float ref = mm == -INFINITY ? 0.f : mm;
-        float ll = l * __expf(m - ref);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) ll += __shfl_xor(ll, o);
+        const float mm = wave_max(m), ref = mm == -INFINITY ? 0.f : mm, ll = wave_sum(l * __expf(m - ref));
         if (lane == 0) ml_s[w] = make_float2(mm, ll), count_s[w] = count;
     }
     __syncthreads();
-    // the four lists joined: a candidate's place is the number of those that come before it
+    if (count_s[0] + count_s[1] + count_s[2] + count_s[3] > 256) {
+        count = wave_keep_best(list, count, n, lane);
+        __syncthreads();
+        if (lane == 0) count_s[w] = count;
+        __syncthreads();
+    }
+    // The four lists joined, and the best n of them: a candidate's place is the number of those that come before it, counted by four threads.  (A thread by itself, which
+    // waits for every LDS read in turn, took 2.6 us of the launch's 8.)
+    const int start = (w > 0 ? count_s[0] : 0) + (w > 1 ? count_s[1] : 0) + (w > 2 ? count_s[2] : 0);
+    const int total = count_s[0] + count_s[1] + count_s[2] + count_s[3];
+    for (int i = lane; i < count; i += 64) flat_s[start + i] = list[i];
+    __syncthreads();
     const long out = ((long)r * slices + p) * n;
-    const int c[4] = {count_s[0], count_s[1], count_s[2], count_s[3]};
-    const int total = c[0] + c[1] + c[2] + c[3];
-    if (lane < c[w]) {
-        const Cand mine = list[lane];
-        int rank = 0;
-        for (int v = 0; v < 4; v++)
-            for (int k = 0; k < c[v]; k++) rank += before(list_s[v][k].x, list_s[v][k].t, mine) ? 1 : 0;
-        if (rank < n) best[out + rank] = mine;
+    for (int i0 = 0; i0 < total; i0 += 64) {
+        const int i = i0 + (threadIdx.x >> 2);
+        const Cand mine = flat_s[min(i, total - 1)];
+        float rank = 0.f;
+#pragma unroll 4
+        for (int k = threadIdx.x & 3; k < total; k += 4) rank += before(flat_s[k].x, flat_s[k].t, mine) ? 1.f : 0.f;
+        rank += dpp_mov<0xB1>(rank);
+        rank += dpp_mov<0x4E>(rank);
+        if (i < total && (threadIdx.x & 3) == 0 && rank < (float)n) best[out + (int)rank] = mine;
     }
     for (int i = total + threadIdx.x; i < n; i += 256) best[out + i] = Cand{-INFINITY, NO_INDEX};
     if (threadIdx.x == 0) {
@@ -201,114 +241,98 @@ struct Scored {
 };
 __device__ __forceinline__ bool before(const Scored& a, const Scored& b) { return a.s > b.s || (a.s == b.s && (a.w < b.w || (a.w == b.w && a.t < b.t))); }
 
-// One workgroup of 16 wavefronts per sequence.  Every slice's list is in order, so of a list whose first entry is not among the n best first entries
-// nothing is wanted: each wavefront finds the n-th best first entry of its share of the lists (by value, rounded down), takes what is no smaller from them,
-// and keeps its best n; then the 16 n are joined.  Scores in double: two beams' candidates may lie closer than floats tell apart.
-constexpr int JOIN_WAVES = 16, JOIN_CAP = 192;
-__global__ __launch_bounds__(64 * JOIN_WAVES) void select_join_kernel(const Cand* __restrict__ best, const float2* __restrict__ part,
-                                                                      const float* __restrict__ scores, int W, int n, int slices,
-                                                                      float* __restrict__ out_s, int* __restrict__ out_w, int* __restrict__ out_t) {
+// One workgroup of 16 wavefronts per sequence on the entries of its beams' slices.  Threshold as above: the largest of the wavefronts' n-th largest lane maxima.  What is
+// no smaller goes into one list, a candidate's place is the number of those that come before it; should they not fit (many equal scores), the n
+// places are filled one by one with the best candidate behind the one before.  Scores in double: two beams' candidates may lie closer than floats
+// tell apart.
+constexpr int JOIN_WAVES = 16, JOIN_THREADS = 64 * JOIN_WAVES, JOIN_CAP = 1024;
+__global__ __launch_bounds__(JOIN_THREADS) void select_join_kernel(const Cand* __restrict__ best, const float2* __restrict__ part,
+                                                                   const float* __restrict__ scores, int W, int n, int slices,
+                                                                   float* __restrict__ out_s, int* __restrict__ out_w, int* __restrict__ out_t) {
     __shared__ double base_s[SELECT_MAX];                        // scores[v] - log of the beam's sum of exp(x - top_s[v])
-    __shared__ float top_s[SELECT_MAX];
-    __shared__ __align__(16) Scored list_s[JOIN_WAVES][JOIN_CAP];
-    __shared__ int count_s[JOIN_WAVES];
+    __shared__ float top_s[SELECT_MAX], thr_s[JOIN_WAVES];
+    __shared__ __align__(16) Scored list_s[JOIN_CAP];
+    __shared__ int count_s;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const long g = blockIdx.x;
+    const int entries = W * slices * n, per_beam = slices * n;
+    const Cand* const mine_in = best + g * entries;
+    Cand c0 = {-INFINITY, NO_INDEX};                             // (on its way while the sums are joined)
+    if ((int)threadIdx.x < entries) c0 = mine_in[threadIdx.x];
+    if (threadIdx.x == 0) count_s = 0;
     for (int v = w; v < W; v += JOIN_WAVES) {
         const float2* pr = part + (g * W + v) * slices;
-        float mm = -INFINITY;
-        for (int i = lane; i < slices; i += 64) mm = fmaxf(mm, pr[i].x);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+        float2 own = {-INFINITY, 0.f};
+        if (lane < slices) own = pr[lane];
+        float mm = own.x;
+        for (int i = lane + 64; i < slices; i += 64) mm = fmaxf(mm, pr[i].x);
+        mm = wave_max(mm);
         const float ref = mm == -INFINITY ? 0.f : mm;
-        double ll = 0.0;
-        for (int i = lane; i < slices; i += 64) ll += (double)pr[i].y * exp((double)pr[i].x - (double)ref);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) ll += __hiloint2double(__shfl_xor(__double2hiint(ll), o), __shfl_xor(__double2loint(ll), o));
+        double ll = (double)own.y * exp((double)own.x - (double)ref);
+        for (int i = lane + 64; i < slices; i += 64) ll += (double)pr[i].y * exp((double)pr[i].x - (double)ref);
+        ll = wave_sum_d(ll);
         if (lane == 0) base_s[v] = (double)scores[g * W + v] - log(ll), top_s[v] = ref;
     }
     __syncthreads();
-    const int lists = W * slices;
-    const int l0 = (int)((long)lists * w / JOIN_WAVES), l1 = (int)((long)lists * (w + 1) / JOIN_WAVES);
-    Scored* const list = list_s[w];
-    int count = 0;
-    auto entry = [&](int li, int k) {
-        const Cand c = best[(g * lists + li) * n + k];
-        const int v = li / slices;
+    auto entry = [&](int e) {
+        const Cand c = e == (int)threadIdx.x ? c0 : mine_in[e];
+        const int v = (unsigned)e / (unsigned)per_beam;
         const double s = base_s[v] + ((double)c.x - (double)top_s[v]);        // (the difference first: both may be the type's lowest value)
         return Scored{s == s && c.t != NO_INDEX ? s : -INFINITY, v, c.t};
     };
-    // (several lanes' maxima of first entries: n different entries are no smaller than the n-th of them)
     float top = -INFINITY;
-    for (int li = l0 + lane; li < l1; li += 64) top = fmaxf(top, (float)entry(li, 0).s);
-    float thr = from_order_bits(wave_nth_bits(order_bits(top), n));
-    if (!(thr == thr)) thr = -INFINITY;
-    auto keep = [&] {
-        wave_lds_sync();
-        Scored mine[JOIN_CAP / 64];
-        int rank[JOIN_CAP / 64];
-#pragma unroll
-        for (int i = 0; i < JOIN_CAP / 64; i++) {
-            const int at = lane + 64 * i;
-            mine[i] = at < count ? list[at] : Scored{0.0, 0, 0};
-            rank[i] = at < count ? 0 : NO_INDEX;
-        }
-        for (int k = 0; k < count; k++) {
-            const Scored o = list[k];
-#pragma unroll
-            for (int i = 0; i < JOIN_CAP / 64; i++) rank[i] += before(o, mine[i]) ? 1 : 0;
-        }
-        wave_lds_sync();
-#pragma unroll
-        for (int i = 0; i < JOIN_CAP / 64; i++)
-            if ((unsigned)rank[i] < (unsigned)n) list[rank[i]] = mine[i];
-        wave_lds_sync();
-        count = min(count, n);
-    };
-    for (int b0 = l0; b0 < l1; b0 += 64) {
-        for (int k = 0; k < n; k++) {                            // entry k of 64 lists
-            bool in = false;
-            Scored e = {-INFINITY, 0, 0};
-            if (b0 + lane < l1) {
-                e = entry(b0 + lane, k);
-                in = e.s > -INFINITY && (float)e.s >= thr;
-            }
-            const uint64_t who = __ballot(in);
-            if (!who) break;                                     // (every list is in order)
-            if (count + 64 > JOIN_CAP) {
-                keep();
-                if (count == n) thr = fmaxf(thr, (float)list[n - 1].s);
-            }
-            if (in) list[count + __popcll(who & ((1ull << lane) - 1))] = e;
-            count += __popcll(who);
-        }
-    }
-    keep();
-    if (lane == 0) count_s[w] = count;
+    for (int e = threadIdx.x; e < entries; e += JOIN_THREADS) top = fmaxf(top, (float)entry(e).s);
+    top = wave_nth(top, n);
+    if (lane == 0) thr_s[w] = top;
     __syncthreads();
-    int total = 0;
+    float thr = thr_s[lane % JOIN_WAVES];
 #pragma unroll
-    for (int v = 0; v < JOIN_WAVES; v++) total += count_s[v];
-    if (lane < count) {
-        const Scored mine = list[lane];
-        int rank = 0;
-        for (int v = 0; v < JOIN_WAVES; v++) {
-            const int cv = count_s[v];
-            for (int k = 0; k < cv; k++) {
-                if (!before(list_s[v][k], mine)) break;          // (in order)
-                rank++;
-            }
-        }
-        if (rank < n) {
-            out_s[g * n + rank] = (float)mine.s;
-            out_w[g * n + rank] = mine.w;
-            out_t[g * n + rank] = mine.t;
+    for (int o = JOIN_WAVES / 2; o > 0; o >>= 1) thr = fmaxf(thr, __shfl_xor(thr, o));
+    for (int e = threadIdx.x; e < entries; e += JOIN_THREADS) {
+        const Scored c = entry(e);
+        if (c.s > -INFINITY && (float)c.s >= thr) {
+            const int at = atomicAdd(&count_s, 1);               // (the order does not matter)
+            if (at < JOIN_CAP) list_s[at] = c;
         }
     }
-    for (int i = total + threadIdx.x; i < n; i += 64 * JOIN_WAVES) {
-        out_s[g * n + i] = -INFINITY;
-        out_w[g * n + i] = -1;
-        out_t[g * n + i] = -1;
+    __syncthreads();
+    const int count = count_s;
+    auto put = [&](int place, const Scored& c) {
+        out_s[g * n + place] = c.w < 0 ? -INFINITY : (float)c.s;
+        out_w[g * n + place] = c.w;
+        out_t[g * n + place] = c.t;
+    };
+    if (count <= JOIN_CAP) {
+        for (int i0 = 0; i0 < count; i0 += JOIN_THREADS / 16) {  // (16 threads count for a candidate)
+            const int i = i0 + (threadIdx.x >> 4);
+            const Scored mine = list_s[min(i, count - 1)];
+            float rank = 0.f;
+            for (int k = threadIdx.x & 15; k < count; k += 16) rank += before(list_s[k], mine) ? 1.f : 0.f;
+            rank = row16_sum(rank);
+            if (i < count && (threadIdx.x & 15) == 0 && rank < (float)n) put((int)rank, mine);
+        }
+        for (int i = count + threadIdx.x; i < n; i += JOIN_THREADS) put(i, Scored{0.0, -1, -1});
+        return;
+    }
+    Scored last = {INFINITY, -1, -1};                            // (count > JOIN_CAP > n: there are n)
+    for (int place = 0; place < n; place++) {
+        __syncthreads();                                         // (the list is read no more, and its first entries hold the wavefronts' best)
+        Scored top1 = {-INFINITY, NO_INDEX, NO_INDEX};
+        for (int e = threadIdx.x; e < entries; e += JOIN_THREADS) {
+            const Scored c = entry(e);
+            if (before(last, c) && before(c, top1)) top1 = c;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const Scored c = {__hiloint2double(__shfl_xor(__double2hiint(top1.s), o), __shfl_xor(__double2loint(top1.s), o)), __shfl_xor(top1.w, o), __shfl_xor(top1.t, o)};
+            if (before(c, top1)) top1 = c;
+        }
+        if (lane == 0) list_s[w] = top1;
+        __syncthreads();
+        last = list_s[0];
+        for (int v = 1; v < JOIN_WAVES; v++)
+            if (before(list_s[v], last)) last = list_s[v];
+        if (threadIdx.x == 0) put(place, last);
     }
 }
 
@@ -381,11 +405,14 @@ __global__ __launch_bounds__(256) void reorder_kernel(const PoolTable pools, con
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// slices of a row: enough wavefronts for every CU to hold eight, but no more than the row has tiles of 4 KiB
-int select_slices(long rows, int V, int elem) {
-    const long tiles = ((long)V * elem + 4095) / 4096, most = (tiles + 3) / 4;
-    const long want = ((long)qt::cu_count() * 2 + rows - 1) / rows;
-    return (int)(want < 1 ? 1 : want < most ? want : most);
+// How a launch cuts its rows: tiles of 4 KiB, tiles a wavefront, workgroups (of four) a row.  Eight workgroups a CU, but no wavefront without a tile.
+struct ScanPlan {
+    unsigned tiles, per_wave, slices;
+};
+ScanPlan scan_plan(long rows, int V, int elem) {
+    const long tiles = ((long)V * elem + 4095) / 4096, waves = std::max(1l, (long)qt::cu_count() * 8 * 4 / rows);
+    const long per = (tiles + waves - 1) / waves;
+    return {(unsigned)tiles, (unsigned)per, (unsigned)((tiles + 4 * per - 1) / (4 * per))};
 }
 
 }  // namespace
@@ -394,7 +421,7 @@ extern "C" {
 
 long qt_beam_select_workspace_bytes(long G, int W, int V, int n, int elem_size) {
     if (G < 0 || W < 1 || W > SELECT_MAX || V < 1 || n < 1 || n > SELECT_MAX || (elem_size != 2 && elem_size != 4) || G * W > 65535) return -1;
-    return G == 0 ? 0 : G * W * select_slices(G * W, V, elem_size) * ((long)n * (long)sizeof(Cand) + (long)sizeof(float2));
+    return G == 0 ? 0 : G * W * scan_plan(G * W, V, elem_size).slices * ((long)n * (long)sizeof(Cand) + (long)sizeof(float2));
 }
 
 int qt_beam_select(const void* logits, int dtype, long stride_g, long stride_w, const float* scores, float* out_scores, int32_t* out_parents,
@@ -407,11 +434,13 @@ int qt_beam_select(const void* logits, int dtype, long stride_g, long stride_w, 
     if (!logits || !scores || !out_scores || !out_parents || !out_tokens || !workspace) return QT_ERR_NULL;
     if (!aligned16(workspace) || (reinterpret_cast<uintptr_t>(logits) & (unsigned)(elem - 1))) return QT_ERR_ALIGN;
     if (workspace_bytes < need) return QT_ERR_WORKSPACE;
-    const int slices = select_slices((long)G * W, V, elem);
+    const ScanPlan plan = scan_plan((long)G * W, V, elem);
+    const int slices = (int)plan.slices;
     float2* const part = (float2*)workspace;
     Cand* const best = (Cand*)(part + (size_t)G * W * slices);
-    const dim3 grid((unsigned)slices, (unsigned)(G * W));
-#define QT_SCAN(T) hipLaunchKernelGGL((select_scan_kernel<T>), grid, dim3(256), 0, stream, (const T*)logits, stride_g, stride_w, W, V, n, slices, best, part)
+    const dim3 grid(plan.slices, (unsigned)W, (unsigned)G);
+#define QT_SCAN(T) hipLaunchKernelGGL((select_scan_kernel<T>), grid, dim3(256), 0, stream, (const T*)logits, stride_g, stride_w, (unsigned)V, n, plan.tiles, \
+                                      plan.per_wave, best, part)
     if (dtype == 0) QT_SCAN(bf16_t);
     else if (dtype == 1) QT_SCAN(f16);
     else QT_SCAN(float);
