@@ -5,6 +5,7 @@
 // its n largest logits and its part (maximum, sum) of l_w; a second launch joins the slices of a sequence's beams.
 #include "qt_common.h"
 #include <algorithm>
+#include <type_traits>
 
 using namespace qt;
 
@@ -97,25 +98,45 @@ __device__ __forceinline__ int wave_keep_best(Cand* list, int count, int n, int 
     return min(count, n);
 }
 
-// the 16 bytes of logits number `piece` of a row; what lies behind the row reads as -inf.  The pieces count from the row's first logit wherever it lies in memory (the
+// A lane's pieces of 16 bytes of a row's tile; what lies behind the row reads as -inf.  The pieces count from the row's first logit wherever it lies in memory (the
 // hardware loads 16 bytes from any element), so that equal rows have equal sums, bit for bit.
+constexpr int PIECES = 4;               // of a lane and tile
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, unsigned piece, unsigned V, float (&x)[16 / sizeof(T)]) {
-    constexpr int N = 16 / sizeof(T);
+__device__ __forceinline__ void load_tile(const T* row, unsigned tile, unsigned V, int lane, u32x4 (&raw)[PIECES]) {
+    constexpr unsigned N = 16 / sizeof(T), TILE = 64 * PIECES;
     typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
-    const unsigned t0 = piece * N;                               // (V < 2^31: no sum passes 2^32)
-    if (t0 + N <= V) {
-        union {
-            u32x4 v;
-            T e[N];
-        } u;
-        u.v = *reinterpret_cast<const words*>(row + t0);
+    const unsigned t0 = (tile * TILE + lane) * N;                // (V < 2^31: no sum passes 2^32)
+    if ((tile + 1) * TILE * N <= V) {                            // (the same for the whole wavefront: with a branch a lane each load was waited for before the next)
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = as_float(u.e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = t0 + i < V ? as_float(row[t0 + i]) : -INFINITY;
+        for (int i = 0; i < PIECES; i++) raw[i] = *reinterpret_cast<const words*>(row + t0 + 64 * i * N);
+        return;
     }
+    constexpr unsigned NONE = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, f16>::value ? 0xfc00fc00u : 0xff80ff80u;      // -inf
+    union {
+        T e[PIECES][N];
+        u32x4 v[PIECES];
+    } u;
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+        u.v[i] = u32x4{NONE, NONE, NONE, NONE};
+#pragma unroll
+        for (unsigned k = 0; k < N; k++) {
+            const unsigned t = t0 + 64 * i * N + k;
+            const T x = row[min(t, V - 1)];
+            if (t < V) u.e[i][k] = x;
+        }
+        raw[i] = u.v[i];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void unpack_piece(u32x4 v, float (&x)[16 / sizeof(T)]) {
+    union {
+        u32x4 v;
+        T e[16 / sizeof(T)];
+    } u;
+    u.v = v;
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); i++) x[i] = as_float(u.e[i]);
 }
 
 // Workgroup (slice p, beam, sequence) of four wavefronts, each on `per_wave` tiles of its own of the beam's row: 64 lanes x 4 pieces of 16 bytes.
@@ -126,7 +147,7 @@ __device__ __forceinline__ void load_piece(const T* row, unsigned piece, unsigne
 template <typename T>
 __global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ logits, long stride_g, long stride_w, unsigned V, int n,
                                                           unsigned tiles, unsigned per_wave, Cand* __restrict__ best, float2* __restrict__ part) {
-    constexpr int N = 16 / sizeof(T), PIECES = 4, TILE = 64 * PIECES;         // pieces a tile
+    constexpr int N = 16 / sizeof(T), TILE = 64 * PIECES;        // pieces a tile
     __shared__ Cand list_s[4][WAVE_CAP], flat_s[256];
     __shared__ int count_s[4];
     __shared__ float thr_s[4];
@@ -145,8 +166,10 @@ __global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ 
         const bool real = tile < last;
         float x[PIECES][N], pm[PIECES];                          // and the pieces' maxima
         if (real) {
+            u32x4 raw[PIECES];
+            load_tile(row, tile, V, lane, raw);
 #pragma unroll
-            for (int i = 0; i < PIECES; i++) load_piece(row, tile * TILE + 64 * i + lane, V, x[i]);
+            for (int i = 0; i < PIECES; i++) unpack_piece<T>(raw[i], x[i]);
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
                 pm[i] = fmaxf(x[i][0], x[i][1]);
@@ -405,12 +428,14 @@ __global__ __launch_bounds__(256) void reorder_kernel(const PoolTable pools, con
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// How a launch cuts its rows: tiles of 4 KiB, tiles a wavefront, workgroups (of four) a row.  Eight workgroups a CU, but no wavefront without a tile.
+// How a launch cuts its rows: tiles of 4 KiB, tiles a wavefront, workgroups (of four) a row.  Sixteen wavefronts a CU, which all fit, but none without a tile (16 x 4 rows of 248320,
+// us with 8 / 16 / 32 a CU: 23.1 / 17.3 / 18.8; a tile's loads
+// ahead of the one before's arithmetic: no difference).
 struct ScanPlan {
     unsigned tiles, per_wave, slices;
 };
 ScanPlan scan_plan(long rows, int V, int elem) {
-    const long tiles = ((long)V * elem + 4095) / 4096, waves = std::max(1l, (long)qt::cu_count() * 8 * 4 / rows);
+    const long tiles = ((long)V * elem + 4095) / 4096, waves = std::max(1l, (long)qt::cu_count() * 16 / rows);
     const long per = (tiles + waves - 1) / waves;
     return {(unsigned)tiles, (unsigned)per, (unsigned)((tiles + 4 * per - 1) / (4 * per))};
 }
