@@ -367,35 +367,39 @@ struct PoolTable {
     u32x4* kv[2 * POOL_LAYERS];
 };
 constexpr int SSM_VEC = HV * DV * DK / 4, CONV_VEC = 3 * CD / 8, KV_VEC = AD / 8;
-constexpr int SSM_UNITS = SSM_VEC / 256, CONV_UNITS = (CONV_VEC + 255) / 256, KV_WGS = 8;
+constexpr int KV_WGS = 8;               // workgroups on the rows of one (pool, sequence, head)
 
 // The state of beam w of sequence g, in slot slots[g][w], becomes that of slot slots[g][parents[g][w]], for all beams of a sequence at once and in place.
 // A thread owns one 16-byte place of the state in all of the sequence's slots: it loads what every beam takes over and stores it, so no beam's
 // old state is overwritten before whoever needs it has read it, whatever the parents are, and nothing is exchanged.  A beam that is its own parent is
 // not touched.  Blocks: ssm (layer, sequence, 4 KiB of a slot), conv (layer, sequence, 4 KiB of the live window), K / V (pool, sequence, head, part of the
 // rows start .. pos - 1).
-template <int WMAX>
+// UN: places a thread loads before it stores the first; stores are nontemporal.  Bound by HBM: 8 x 4 beams of 24 layers, 1200 rows of the caches, move 1.54 GB in 313 us
+// (4.9 TB/s, a large copy reaches 5.2).  us at 1 x 4 / 8 x 4 beams: one place with plain stores 19.2 / 324, nontemporal stores 18.4 / 314, two places 17.9 /
+// 313, four 19.3 / 317; nontemporal loads lose what two beams take from one parent (22.3 / 312).
+template <int WMAX, int UN>
 __global__ __launch_bounds__(256) void reorder_kernel(const PoolTable pools, const int* __restrict__ slots, const int* __restrict__ parents,
                                                       const int* __restrict__ start, const int* __restrict__ pos, int G, int W, int n_ssm, int n_slots,
                                                       int Lmax) {
+    constexpr unsigned SSM_UNITS = SSM_VEC / (256 * UN), CONV_UNITS = (CONV_VEC + 256 * UN - 1) / (256 * UN);
     const unsigned ssm_blocks = (unsigned)n_ssm * G * SSM_UNITS, conv_blocks = (unsigned)n_ssm * G * CONV_UNITS;
     unsigned id = blockIdx.x;
     u32x4* base;
     size_t slot_stride;                                          // vectors from a slot to the next
     long first, end;                                             // this thread's first place, and the end of the places
-    int step, g;
+    int step = 256, g;                                           // between a thread's places
     if (id < ssm_blocks) {
         const unsigned unit = id % SSM_UNITS, lg = id / SSM_UNITS;
         g = lg % G;
         base = pools.ssm[lg / G];
         slot_stride = SSM_VEC;
-        first = unit * 256 + threadIdx.x, end = SSM_VEC, step = SSM_VEC;
+        first = unit * (256 * UN) + threadIdx.x, end = (unit + 1) * (256 * UN);
     } else if ((id -= ssm_blocks) < conv_blocks) {
         const unsigned unit = id % CONV_UNITS, lg = id / CONV_UNITS;
         g = lg % G;
         base = pools.conv[lg / G] + (pos[g] & 1) * CONV_VEC;
         slot_stride = 2 * CONV_VEC;
-        first = unit * 256 + threadIdx.x, end = CONV_VEC, step = CONV_VEC;
+        first = unit * (256 * UN) + threadIdx.x, end = min((unit + 1) * (256 * UN), (unsigned)CONV_VEC);
     } else {
         id -= conv_blocks;
         const unsigned part = id % KV_WGS, head = id / KV_WGS % AKV, pg = id / KV_WGS / AKV;
@@ -415,14 +419,18 @@ __global__ __launch_bounds__(256) void reorder_kernel(const PoolTable pools, con
             if ((unsigned)from[w] >= (unsigned)n_slots) from[w] = -1;
         }
     }
-    for (long at = first; at < end; at += step) {
-        u32x4 v[WMAX];
+    for (long at = first; at < end; at += (long)UN * step) {
+        u32x4 v[UN][WMAX];
 #pragma unroll
-        for (int w = 0; w < WMAX; w++)
-            if (from[w] >= 0) v[w] = base[(size_t)from[w] * slot_stride + at];
+        for (int u = 0; u < UN; u++)
 #pragma unroll
-        for (int w = 0; w < WMAX; w++)
-            if (from[w] >= 0) base[(size_t)to[w] * slot_stride + at] = v[w];
+            for (int w = 0; w < WMAX; w++)
+                if (from[w] >= 0 && at + (long)u * step < end) v[u][w] = base[(size_t)from[w] * slot_stride + at + (long)u * step];
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+#pragma unroll
+            for (int w = 0; w < WMAX; w++)
+                if (from[w] >= 0 && at + (long)u * step < end) __builtin_nontemporal_store(v[u][w], base + (size_t)to[w] * slot_stride + at + (long)u * step);
     }
 }
 
@@ -498,14 +506,15 @@ int qt_beam_reorder(float* const* ssm_pool, void* const* conv_pool, int n_gdn, v
         for (int i = 0; i < na; i++) t.ssm[i] = (u32x4*)ssm_pool[a + i], t.conv[i] = (u32x4*)conv_pool[a + i];
         for (int i = 0; i < nk; i++) t.kv[i] = (u32x4*)kv_pool[k + i];
         a += na, k += nk;
-        const long blocks = (long)na * G * (SSM_UNITS + CONV_UNITS) + (long)nk * G * AKV * KV_WGS;
+        const int un = W <= 4 ? 2 : W <= 8 ? 2 : 1, per = 256 * un;
+        const long blocks = (long)na * G * (SSM_VEC / per + (CONV_VEC + per - 1) / per) + (long)nk * G * AKV * KV_WGS;
         if (blocks > 0x7fffffffl) return QT_ERR_DIM;
-#define QT_REORDER(WM) \
-    hipLaunchKernelGGL((reorder_kernel<WM>), dim3((unsigned)blocks), dim3(256), 0, stream, t, slots, parents, start, pos, G, W, na, n_slots, Lmax)
-        if (W <= 4) QT_REORDER(4);
-        else if (W <= 8) QT_REORDER(8);
-        else if (W <= 16) QT_REORDER(16);
-        else QT_REORDER(32);
+#define QT_REORDER(WM, UN) \
+    hipLaunchKernelGGL((reorder_kernel<WM, UN>), dim3((unsigned)blocks), dim3(256), 0, stream, t, slots, parents, start, pos, G, W, na, n_slots, Lmax)
+        if (W <= 4) QT_REORDER(4, 2);
+        else if (W <= 8) QT_REORDER(8, 2);
+        else if (W <= 16) QT_REORDER(16, 1);
+        else QT_REORDER(32, 1);
 #undef QT_REORDER
         QT_CHECK_LAUNCH();
     }
