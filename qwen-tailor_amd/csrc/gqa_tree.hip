@@ -10,7 +10,9 @@
 //            which spreads the 16 rows of a fragment over the banks
 //   scores : S^T[32 keys x 16 rows] = K . Q^T (16x16x32 bf16 MFMA); a row tile is four tokens x the four heads of the KV head; Q^T stays in registers
 //   P . V  : O^T[256 x 16 rows] += V^T . P^T, V^T through the transposing LDS load
-// Eight wavefronts: row tiles, and where there are few, key halves (KG) and halves of the 256 columns (CG) go to different ones.
+// Eight wavefronts: each takes row tiles of its own; where there are fewer than eight, CG of them share a row tile's scores and take 256 / CG columns of O
+// each.  (Key halves instead would need half the score products, but a partial result each.)
+// A visit to a segment is prepared while the one before is finished: its first tiles are asked for ahead of the stores of the partial result.
 #include "tree.h"
 
 using namespace qt;
@@ -25,7 +27,7 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int GQA = AH / AKV, QKV_W = AH * 2 * AD + 2 * AKV * AD;
 constexpr int KT = 32, ROW_BYTES = AD * 2, TILE_BYTES = KT * ROW_BYTES;        // keys a tile; bytes of its K (or V)
-constexpr int BUFS = 4, WAVES = 8, THREADS = 64 * WAVES;
+constexpr int BUFS = 4, AHEAD = BUFS - 1, WAVES = 8, THREADS = 64 * WAVES;
 constexpr float SCALE_LOG2E = 0.0625f * 1.44269504088896f;                     // 256^-0.5 log2(e): the softmax works with powers of two
 constexpr float NEG = -3.0e38f;
 constexpr int MAX_SEG = 2048, MAX_GRID = 1024;
@@ -70,14 +72,33 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// RT row tiles a wavefront; NRG = 8 / (KG CG) groups of wavefronts with rows of their own
-template <int RT, int KG, int CG>
+// inclusive prefix sum over the wavefront's lanes: four shifts within each 16-lane row, then the rows' totals as scalars
+__device__ __forceinline__ int wave_prefix_sum(int v, int lane) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);           // row_shr:1, 2, 4, 8 (zeros shifted in)
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
+    return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r0 + r1 : r0 + r1 + r2);
+}
+// A direct-to-LDS load of 16 bytes per lane from a scalar address and a lane's 32-bit offset; the 64 pieces land at lds + 16 l.  Inline assembly: waited for by hand.
+// Nontemporal: a tile is read once, and plain loads of it stream at 3.3 TB/s, these at more than 6 (16 sequences of 1024 - 8192 keys, no arithmetic).
+__device__ __forceinline__ void lds_dma16_at(const void* base, unsigned off, unsigned lds) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
+}
+
+// RT row tiles a wavefront, NRG = 8 / CG groups of wavefronts with rows of their own
+template <int RT, int CG>
 __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_new,
                                                                const bf16_t* __restrict__ v_new, bf16_t* Kp, bf16_t* Vp,
                                                                const int* __restrict__ slots, const int* __restrict__ pos,
                                                                const int* __restrict__ parents, float* __restrict__ part_o,
                                                                float* __restrict__ part_ml, int* __restrict__ seg_tab, const Plan plan) {
-    constexpr int NRG = WAVES / (KG * CG), ROWS = 16 * RT * NRG, KW = KT / KG, CB = 16 / CG;   // rows; keys of a tile and column blocks a wavefront takes
+    constexpr int NRG = WAVES / CG, ROWS = 16 * RT * NRG, CB = 16 / CG;      // rows; column blocks a wavefront takes
     // P as two bf16 terms (off by 2^-17) while the launch is bound by the cache's bytes.  With two row tiles a wavefront the second product would cost a half
     // more MFMA time: P is rounded once (2^-9 of each weight, the sum is taken of the rounded ones), less than the output's own rounding.
     constexpr bool SPLIT = RT == 1;
@@ -86,22 +107,26 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
     __shared__ uint64_t seen_s[TREE_MAX];                        // bit i of entry j: token j sees new key i
     __shared__ unsigned bad_s[2];
     const int M = plan.M, nseg = plan.B * AKV;
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int rg = w / (KG * CG), kg = w / CG % KG, cg = w % CG;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int rg = w / CG, cg = w % CG;
 
-    // ends of the segments in the flat space
-    {
+    // Ends of the segments in the flat space.  Up to 64 segments: in every wavefront's lanes, with their slots and positions, without a barrier
+    int lane_end = 0, lane_slot = 0, lane_pos = 0, total;
+    if (nseg <= 64) {
+        if (lane < nseg) lane_slot = slots[lane / AKV], lane_pos = pos[lane / AKV];
+        lane_end = wave_prefix_sum(segment_tiles(plan, lane < nseg ? lane_slot : -1, lane_pos), lane);
+        total = __builtin_amdgcn_readlane(lane_end, 63);
+        if (blockIdx.x == 0 && w == 0) {                         // (the merge kernel reads the table)
+            if (lane == 0) seg_tab[0] = 0;
+            if (lane < nseg) seg_tab[lane + 1] = lane_end;
+        }
+    } else {
         __shared__ int wave_total[WAVES];
         int carry = 0;
-        if (tid == 0) seg_start[0] = 0;
+        if (threadIdx.x == 0) seg_start[0] = 0;
         for (int base = 0; base < nseg; base += THREADS) {
-            const int sg = base + tid;
-            int v = sg < nseg ? segment_tiles(plan, slots[sg / AKV], pos[sg / AKV]) : 0;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int u = __shfl_up(v, o);
-                if (lane >= o) v += u;
-            }
+            const int sg = base + threadIdx.x;
+            const int v = wave_prefix_sum(sg < nseg ? segment_tiles(plan, slots[sg / AKV], pos[sg / AKV]) : 0, lane);
             if (lane == 63) wave_total[w] = v;
             __syncthreads();
             int before = carry;
@@ -113,94 +138,115 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
             __syncthreads();
         }
         if (blockIdx.x == 0)
-            for (int i = tid; i <= nseg; i += THREADS) seg_tab[i] = seg_start[i];
+            for (int i = threadIdx.x; i <= nseg; i += THREADS) seg_tab[i] = seg_start[i];
+        total = __builtin_amdgcn_readfirstlane(seg_start[nseg]);
     }
-    const int total = __builtin_amdgcn_readfirstlane(seg_start[nseg]);
+    auto end_of = [&](int sg) { return sg < 0 ? 0 : nseg <= 64 ? __builtin_amdgcn_readlane(lane_end, sg) : __builtin_amdgcn_readfirstlane(seg_start[sg + 1]); };
     const int per = tiles_per_wg(total, gridDim.x, plan.min_tiles);
     const int wt0 = blockIdx.x * per, wt1 = min(wt0 + per, total);
     if (wt0 >= wt1) return;
     int sg = 0;                                                  // the segment that holds position wt0
-    for (int hi = nseg; sg < hi;) {
-        const int mid = (sg + hi) >> 1;
-        if (__builtin_amdgcn_readfirstlane(seg_start[mid + 1]) <= wt0) sg = mid + 1; else hi = mid;
+    if (nseg <= 64) {
+        sg = __popcll(__ballot(lane < nseg && lane_end <= wt0));
+    } else {
+        for (int hi = nseg; sg < hi;) {
+            const int mid = (sg + hi) >> 1;
+            if (end_of(mid) <= wt0) sg = mid + 1; else hi = mid;
+        }
     }
     const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)tile_s);
 
-    for (; sg < nseg; sg++) {
-        const int begin = __builtin_amdgcn_readfirstlane(seg_start[sg]), end = __builtin_amdgcn_readfirstlane(seg_start[sg + 1]);
-        if (begin + plan.visit >= wt1) break;
-        if (end == begin || end <= wt0) continue;
-        const int b = sg / AKV, kvh = sg % AKV, slot = slots[b], p0 = pos[b];
-        const int pool_tiles = (p0 + KT - 1) / KT;
-        const int t0 = max(wt0 - begin - plan.visit, 0), t1 = min(wt1, end) - begin - plan.visit;      // tiles of the segment
-        const size_t pool_at = ((size_t)slot * AKV + kvh) * plan.Lmax * AD;
-        const bf16_t* const kn = k_new + ((size_t)b * M * AKV + kvh) * AD;
-        const bf16_t* const vn = v_new + ((size_t)b * M * AKV + kvh) * AD;
-
-        // rows w, w + 8, .. of pairs of a tile's rows: lane l brings place l & 31 of row 2 i + (l >> 5)
-        auto issue = [&](int t) {
-            const unsigned buf = lds0 + (unsigned)(t & (BUFS - 1)) * (2 * TILE_BYTES);
-            const int ln = opaque(lane);
-#pragma unroll
-            for (int i = 0; i < KT / 2 / WAVES; i++) {
-                const int r = 2 * (w + WAVES * i) + (ln >> 5), piece = (ln & 31) ^ (r & 15);
-                size_t at;
-                const bf16_t *ks, *vs;
-                if (t < pool_tiles) {                            // (a key past the end: the tile's first one instead, its weight is 0)
-                    const int key = t * KT + r < p0 ? t * KT + r : t * KT;
-                    at = pool_at + (size_t)key * AD;
-                    ks = Kp, vs = Vp;
-                } else {
-                    at = (size_t)min((t - pool_tiles) * KT + r, M - 1) * (AKV * AD);
-                    ks = kn, vs = vn;
-                }
-                const unsigned to = buf + (unsigned)(w + WAVES * i) * (2 * ROW_BYTES);
-                lds_dma16_from(reinterpret_cast<const char*>(ks + at) + 16 * piece, to);
-                lds_dma16_from(reinterpret_cast<const char*>(vs + at) + 16 * piece, to + TILE_BYTES);
-            }
-        };
-        constexpr int PER_TILE = KT / WAVES;                     // loads a wavefront issues per tile
-        // Q^T: lane (row n, group g) holds q[row n][32 kb + 8 g .. + 8] of each row tile
-        bf16x8 bq[RT][8];
-        {
-            const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
-#pragma unroll
-            for (int t = 0; t < RT; t++) {
-                const int tok = (rg * RT + t) * 4 + n / GQA;
-                const bf16_t* qr = q + ((size_t)(b * M + min(tok, M - 1)) * AH + kvh * GQA + n % GQA) * AD;
-#pragma unroll
-                for (int kb = 0; kb < 8; kb++) {
-                    u32x4 x = reinterpret_cast<const u32x4*>(qr)[kb * 4 + g];
-                    if (tok >= M) x = u32x4{0, 0, 0, 0};
-                    bq[t][kb] = __builtin_bit_cast(bf16x8, x);
-                }
-            }
+    // A visit: the part of one segment's tiles that lies in this workgroup's range.  All of it is scalar.
+    struct Visit {
+        int sg, slot, p0, t0, t1;                                // sg < 0: there is none
+    };
+    auto find_visit = [&](int s) {                               // the first one at or after segment s
+        Visit v = {-1, 0, 0, 0, 0};
+        for (; s < nseg; s++) {
+            const int begin = end_of(s - 1), end = end_of(s);
+            if (begin + plan.visit >= wt1) break;
+            if (end == begin || end <= wt0) continue;            // (a skipped sequence)
+            v.sg = s;
+            v.slot = nseg <= 64 ? __builtin_amdgcn_readlane(lane_slot, s) : __builtin_amdgcn_readfirstlane(slots[s / AKV]);
+            v.p0 = nseg <= 64 ? __builtin_amdgcn_readlane(lane_pos, s) : __builtin_amdgcn_readfirstlane(pos[s / AKV]);
+            v.t0 = max(wt0 - begin - plan.visit, 0), v.t1 = min(wt1, end) - begin - plan.visit;
+            break;
         }
-        if (w == 0) seen_s[lane] = tree_ancestors(tree_parent(parents + (size_t)b * M, lane, M), lane);
-        if (w == 0 && lane < 2) bad_s[lane] = 0;
-        __syncthreads();                                         // (also: the visit before is done with the tiles)
-        for (int i = 0; i < BUFS - 1; i++)
-            if (t0 + i < t1) issue(t0 + i);
+        return v;
+    };
+    auto pool_rows = [&](const Visit& v) { return ((size_t)v.slot * AKV + v.sg % AKV) * plan.Lmax * AD; };
+    auto new_rows = [&](const Visit& v) { return ((size_t)(v.sg / AKV) * M * AKV + v.sg % AKV) * AD; };
+    // Wavefront w brings the row pairs w and w + 8 of a tile: lane l place l & 31 of row 2 i + (l >> 5)
+    constexpr int PAIRS = KT / 2 / WAVES, PER_TILE = 2 * PAIRS;  // and issues so many loads for it
+    auto issue = [&](const Visit& v, int t) {
+        const unsigned buf = lds0 + (unsigned)(t & (BUFS - 1)) * (2 * TILE_BYTES);
+        const int pool_tiles = (v.p0 + KT - 1) / KT;
+        const bool is_new = t >= pool_tiles;
+        const int key0 = (is_new ? t - pool_tiles : t) * KT, left = (is_new ? M : v.p0) - key0;
+        const size_t at = is_new ? new_rows(v) + (size_t)key0 * (AKV * AD) : pool_rows(v) + (size_t)key0 * AD;
+        const bf16_t *ks = (is_new ? k_new : Kp) + at, *vs = (is_new ? v_new : Vp) + at;
+        const int ln = opaque(lane);
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) {
+            int r = 2 * (w + WAVES * i) + (ln >> 5);
+            const unsigned piece = (ln & 31) ^ (r & 15);
+            if (left < KT) r = min(r, left - 1);                 // (a key past the end: the last one instead, its weight is 0)
+            const unsigned off = (unsigned)r * (is_new ? AKV * ROW_BYTES : ROW_BYTES) + 16 * piece;
+            const unsigned to = buf + (unsigned)(w + WAVES * i) * (2 * ROW_BYTES);
+            lds_dma16_at(ks, off, __builtin_amdgcn_readfirstlane(to));
+            lds_dma16_at(vs, off, __builtin_amdgcn_readfirstlane(to + TILE_BYTES));
+        }
+    };
 
+    Visit v = find_visit(sg);
+    if (v.sg < 0) return;
+    bf16x8 bq[RT][8];
+    auto load_q = [&] {                                          // Q^T: lane (row n, group g) holds q[row n][32 kb + 8 g .. + 8] of each row tile
+        const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int tok = min((rg * RT + t) * 4 + n / GQA, M - 1);          // (rows past the last token repeat it; they are not stored)
+            const u32x4* qr = reinterpret_cast<const u32x4*>(q + ((size_t)(v.sg / AKV * M + tok) * AH + v.sg % AKV * GQA + n % GQA) * AD);
+#pragma unroll
+            for (int kb = 0; kb < 8; kb++) bq[t][kb] = __builtin_bit_cast(bf16x8, qr[kb * 4 + g]);
+        }
+    };
+    load_q();
+    __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < AHEAD; i++)
+        if (v.t0 + i < v.t1) issue(v, v.t0 + i);
+    while (true) {
+        const int pool_tiles = (v.p0 + KT - 1) / KT;
+        const bool has_new = v.t1 > pool_tiles;
+        if (has_new && w == 0) {
+            if (lane < 2) bad_s[lane] = 0;
+            seen_s[lane] = tree_ancestors(tree_parent(parents + (size_t)(v.sg / AKV) * M, lane, M), lane);
+        }
+        // q is waited for here: in the tile loop the compiler would wait for its loads in every turn, and for the tiles in flight with them
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int kb = 0; kb < 8; kb++) asm volatile("" : "+v"(bq[t][kb]));
         f32x4 O[RT][CB];
-        float m_run[RT], l_run[RT];
+        float m_run[RT], l_run[RT];                              // reference points (in the units of the raw products), sums
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             m_run[t] = NEG, l_run[t] = 0.f;
 #pragma unroll
             for (int j = 0; j < CB; j++) O[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        for (int tile = t0; tile < t1; tile++) {
-            const int ahead = t1 - 1 - tile;                     // tiles that are in flight behind this one
+        for (int tile = v.t0; tile < v.t1; tile++) {
+            const int ahead = v.t1 - 1 - tile;                   // tiles that are in flight behind this one
             if (ahead >= 2) wait_vmem<2 * PER_TILE>();
             else if (ahead == 1) wait_vmem<PER_TILE>();
             else wait_vmem<0>();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             barrier();                                           // everyone's part of the tile has landed, and everyone is done with the buffer filled next
-            if (tile + BUFS - 1 < t1) issue(tile + BUFS - 1);
+            if (tile + AHEAD < v.t1) issue(v, tile + AHEAD);
             const unsigned char* const kt = tile_s + (tile & (BUFS - 1)) * (2 * TILE_BYTES);
             unsigned char* const vt = tile_s + (tile & (BUFS - 1)) * (2 * TILE_BYTES) + TILE_BYTES;
             const bool is_new = tile >= pool_tiles;
-            const int key0 = is_new ? (tile - pool_tiles) * KT : tile * KT, keys = is_new ? M : p0;
+            const int key0 = is_new ? (tile - pool_tiles) * KT : tile * KT, keys = is_new ? M : v.p0;
             if (is_new) {
                 // A new value that is not finite must not reach rows that do not see it (0 times NaN): it becomes 0 here, and rows that do
                 // see its token become NaN at the end.  Rows past the last token become 0.
@@ -217,12 +263,11 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                 __syncthreads();
             }
             const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
-            f32x4 s[RT][KW / 16];
+            f32x4 s[RT][KT / 16];
 #pragma unroll
-            for (int u = 0; u < KW / 16; u++) {
+            for (int u = 0; u < KT / 16; u++) {
                 if (RT > 1) __builtin_amdgcn_sched_barrier(0);
-                const int row = kg * KW + 16 * u + n;            // A operand: lane (key n, group g) holds k[key][32 kb + 8 g .. + 8]
-                const unsigned at = row * ROW_BYTES + ((g ^ n) << 4);
+                const unsigned at = (16 * u + n) * ROW_BYTES + ((g ^ n) << 4);     // A operand: lane (key n, group g) holds k[key][32 kb + 8 g .. + 8]
 #pragma unroll
                 for (int t = 0; t < RT; t++) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -233,35 +278,38 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                     for (int t = 0; t < RT; t++) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, bq[t][kb], s[t][u], 0, 0, 0);
                 }
             }
-            // online softmax: lane (row n, group g) holds keys 16 u + 4 g .. + 3
+            // online softmax on the raw products: lane (row n, group g) holds keys 16 u + 4 g .. + 3
             const bool masked = is_new || key0 + KT > keys;
-            u32x2 ph[RT][KW / 16], pl[SPLIT ? RT : 1][KW / 16];
+            u32x2 ph[RT][KT / 16], pl[SPLIT ? RT : 1][KT / 16];
 #pragma unroll
             for (int t = 0; t < RT; t++) {
-                float mx = NEG;
-                const uint64_t seen = is_new ? seen_s[((rg * RT + t) * 4 + n / GQA) & 63] : 0;
+                if (masked) {
+                    const uint64_t seen = is_new ? seen_s[((rg * RT + t) * 4 + n / GQA) & 63] : 0;
 #pragma unroll
-                for (int u = 0; u < KW / 16; u++)
+                    for (int u = 0; u < KT / 16; u++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        float x = s[t][u][i] * SCALE_LOG2E;
-                        if (masked) {
-                            const int key = key0 + kg * KW + 16 * u + 4 * g + i;
+                        for (int i = 0; i < 4; i++) {
+                            const int key = key0 + 16 * u + 4 * g + i;
                             const bool on = is_new ? key < M && (seen >> (key & 63) & 1) : key < keys;
-                            x = on ? x : NEG;
+                            s[t][u][i] = on ? s[t][u][i] : NEG;
                         }
-                        s[t][u][i] = x;
-                        mx = fmaxf(mx, x);
-                    }
+                }
+                float mx = fmaxf(s[t][0][0], s[t][0][1]);
+#pragma unroll
+                for (int u = 0; u < KT / 16; u++)
+#pragma unroll
+                    for (int i = u == 0 ? 2 : 0; i < 4; i += 2) mx = fmaxf(fmaxf(mx, s[t][u][i]), s[t][u][i + 1]);
                 mx = max_over_groups(mx);
-                const float m_new = fmaxf(m_run[t], mx), corr = __builtin_amdgcn_exp2f(m_run[t] - m_new);
+                // (the reference point moves only when the maximum has grown by more than 2^8: O is rarely rescaled)
+                const float m_new = mx > m_run[t] + 8.f / SCALE_LOG2E ? mx : m_run[t], mc = m_new * SCALE_LOG2E;
+                const float corr = __builtin_amdgcn_exp2f((m_run[t] - m_new) * SCALE_LOG2E);
                 float sum = 0.f;
 #pragma unroll
-                for (int u = 0; u < KW / 16; u++) {
+                for (int u = 0; u < KT / 16; u++) {
                     float p[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        p[i] = __builtin_amdgcn_exp2f(s[t][u][i] - m_new);
+                        p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], SCALE_LOG2E, -mc));
                         if (masked && s[t][u][i] <= 0.5f * NEG) p[i] = 0.f;
                         if constexpr (SPLIT) sum += p[i];
                     }
@@ -279,41 +327,39 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                     for (int j = 0; j < CB; j++) O[t][j] *= corr;
                 }
             }
-            // transposing load: lane (n, g) points at key 4 g + n / 4, columns 4 (n % 4) .. + 3 of the block, and receives keys 4 g .. + 3 of column n
-            const int vkey = kg * KW + 4 * g + (n >> 2);
-            const unsigned vat = vkey * ROW_BYTES + ((((n >> 1) & 1) ^ (vkey & 15)) << 4) + (n & 1) * 8;
+            // transposing load: lane (n, g) points at key 4 g + n / 4, columns 4 (n % 4) .. + 3 of the block, and receives keys 4 g .. + 3 of column n.  Two of them are
+            // the A operand when the 32 keys are enumerated as 16 (e >> 2) + 4 g + (e & 3), in which order the lane holds its probabilities.
+            const int vkey = 4 * g + (n >> 2);
+            const unsigned vat = vkey * ROW_BYTES + ((((n >> 1) & 1) ^ vkey) << 4) + (n & 1) * 8;
 #pragma unroll
             for (int j = 0; j < CB; j++) {
                 if (RT > 1 && j % 4 == 0) __builtin_amdgcn_sched_barrier(0);    // (at most four column blocks' fragments in registers at a time)
-                s16x4 a[KW / 16];
+                s16x4 a[2];
 #pragma unroll
-                for (int u = 0; u < KW / 16; u++)
+                for (int u = 0; u < 2; u++)
                     a[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                         (__attribute__((address_space(3))) s16x4*)(vt + (vat ^ ((cg * CB + j) << 5)) + u * 16 * ROW_BYTES));
-                if constexpr (KW == 32) {
-                    const s16x4 a0 = a[0], a1 = a[1];
-                    const bf16x8 av = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+                const s16x4 a0 = a[0], a1 = a[1];
+                const bf16x8 av = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        const u32x4 hp = {ph[t][0][0], ph[t][0][1], ph[t][1][0], ph[t][1][1]};
-                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, hp), O[t][j], 0, 0, 0);
-                        if constexpr (SPLIT) {
-                            const u32x4 lp = {pl[t][0][0], pl[t][0][1], pl[t][1][0], pl[t][1][1]};
-                            O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, lp), O[t][j], 0, 0, 0);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a[0], __builtin_bit_cast(s16x4, ph[t][0]), O[t][j], 0, 0, 0);
-                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a[0], __builtin_bit_cast(s16x4, pl[t][0]), O[t][j], 0, 0, 0);
+                for (int t = 0; t < RT; t++) {
+                    const u32x4 hp = {ph[t][0][0], ph[t][0][1], ph[t][1][0], ph[t][1][1]};
+                    O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, hp), O[t][j], 0, 0, 0);
+                    if constexpr (SPLIT) {
+                        const u32x4 lp = {pl[t][0][0], pl[t][0][1], pl[t][1][0], pl[t][1][1]};
+                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, lp), O[t][j], 0, 0, 0);
                     }
                 }
             }
         }
-        // partial results of this visit, one per key group: [slot][ROWS][256] and (maximum, sum)
-        const uint64_t bad = (uint64_t)bad_s[1] << 32 | bad_s[0];
-        const size_t at = ((size_t)blockIdx.x + sg) * KG + kg;
+        const Visit next = find_visit(v.sg + 1);
+        __syncthreads();                                         // everyone is done with the tiles, and has said what is not finite
+        if (next.sg >= 0)
+            for (int i = 0; i < AHEAD; i++)
+                if (next.t0 + i < next.t1) issue(next, next.t0 + i);
+        // the partial result of this visit: [ROWS][256], and per row (reference point in powers of two, sum)
+        const uint64_t bad = has_new ? (uint64_t)bad_s[1] << 32 | bad_s[0] : 0;
+        const size_t at = (size_t)blockIdx.x + v.sg;
         {
             const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
 #pragma unroll
@@ -325,21 +371,27 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
 #pragma unroll
                     for (int j = 0; j < CB; j++) *reinterpret_cast<f32x4*>(po + 16 * j) = O[t][j];
                     if (g == 0 && cg == 0) {
-                        part_ml[(at * ROWS + row) * 2] = m_run[t];
-                        part_ml[(at * ROWS + row) * 2 + 1] = seen_s[tok] & bad ? __builtin_nanf("") : l;
+                        part_ml[(at * ROWS + row) * 2] = m_run[t] * SCALE_LOG2E;
+                        part_ml[(at * ROWS + row) * 2 + 1] = bad && (seen_s[tok] & bad) ? __builtin_nanf("") : l;
                     }
                 }
             }
         }
         // the new rows of this visit's tiles go into the pool (nobody reads it from pos on)
-        for (int i = 64 * w + opaque(lane) + max(t0 - pool_tiles, 0) * KT * 32, e = min((t1 - pool_tiles) * KT, M) * 32; i < e; i += THREADS) {
-            const int key = i / 32, c = i % 32;
-            const size_t to = (pool_at + (size_t)(p0 + key) * AD) / 8 + c, from = (size_t)key * (AKV * AD / 8) + c;
-            const u32x4 kx = reinterpret_cast<const u32x4*>(kn)[from], vx = reinterpret_cast<const u32x4*>(vn)[from];
-            reinterpret_cast<u32x4*>(Kp)[to] = kx;
-            reinterpret_cast<u32x4*>(Vp)[to] = vx;
+        if (has_new) {
+            const bf16_t *kn = k_new + new_rows(v), *vn = v_new + new_rows(v);
+            for (int i = 64 * w + opaque(lane) + max(v.t0 - pool_tiles, 0) * KT * 32, e = min((v.t1 - pool_tiles) * KT, M) * 32; i < e; i += THREADS) {
+                const int key = i / 32, c = i % 32;
+                const size_t to = (pool_rows(v) + (size_t)(v.p0 + key) * AD) / 8 + c, from = (size_t)key * (AKV * AD / 8) + c;
+                const u32x4 kx = reinterpret_cast<const u32x4*>(kn)[from], vx = reinterpret_cast<const u32x4*>(vn)[from];
+                reinterpret_cast<u32x4*>(Kp)[to] = kx;
+                reinterpret_cast<u32x4*>(Vp)[to] = vx;
+            }
         }
+        if (next.sg < 0) break;
         __syncthreads();                                         // (the next visit clears what this one has collected)
+        v = next;
+        load_q();
     }
 }
 
@@ -348,7 +400,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
 template <bool GATE>
 __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                               const int* __restrict__ seg_tab, bf16_t* __restrict__ out, const bf16_t* __restrict__ qkv,
-                                                              int nwg, int rows, int KG, const Plan plan) {
+                                                              int nwg, int rows, const Plan plan) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int id = blockIdx.x * 4 + w;
     if (id >= plan.B * plan.M * AH) return;
@@ -359,8 +411,8 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     float l = 1.f;
     if (se > ss) {
         const int per = tiles_per_wg(total, nwg, plan.min_tiles);
-        const int wg0 = (ss + plan.visit) / per, ns = ((se - 1) / per - wg0 + 1) * KG;
-        const size_t at = ((size_t)wg0 + sg) * KG;
+        const int wg0 = (ss + plan.visit) / per, ns = (se - 1) / per - wg0 + 1;
+        const size_t at = (size_t)wg0 + sg;
         const float* ml = part_ml + (at * rows + row) * 2;
         const float* po = part_o + (at * rows + row) * AD + 4 * lane;
         float mm = NEG;
@@ -406,37 +458,31 @@ inline int grid_size() {
     const int cus = qt::cu_count();
     return cus < MAX_GRID ? cus : MAX_GRID;
 }
-// rows of a partial result, and key groups
-inline void shape(int M, int& rows, int& kg) {
-    rows = M <= 8 ? 32 : M <= 16 ? 64 : M <= 32 ? 128 : 256;
-    kg = M <= 16 ? 2 : 1;
-}
+inline int partial_rows(int M) { return M <= 8 ? 32 : M <= 16 ? 64 : M <= 32 ? 128 : 256; }
 constexpr long SEG_TAB_BYTES = ((MAX_SEG + 1) * 4 + 15) / 16 * 16;
 
 int launch(const void* q, const void* k, const void* v, void* Kp, void* Vp, const int32_t* slots, const int32_t* pos, const int32_t* parents, void* out,
            const void* gate_rows, void* workspace, int B, int M, int Lmax, int n_slots, hipStream_t stream) {
-    int rows, kg;
-    shape(M, rows, kg);
-    const int nwg = grid_size();
-    const size_t cap = ((size_t)nwg + (size_t)B * AKV) * kg;
+    const int rows = partial_rows(M), nwg = grid_size();
+    const size_t cap = (size_t)nwg + (size_t)B * AKV;
     float* const part_o = (float*)workspace;
     float* const part_ml = part_o + cap * rows * AD;
     int* const seg_tab = reinterpret_cast<int*>(part_ml + cap * rows * 2);
     const Plan plan = {B, M, Lmax, n_slots, 2 + rows / 64, 2};
-#define QT_TREE_ATTN(RT, KG, CG)                                                                                                                       \
-    hipLaunchKernelGGL((attn_tree_kernel<RT, KG, CG>), dim3((unsigned)nwg), dim3(THREADS), 0, stream, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, \
+#define QT_TREE_ATTN(RT, CG)                                                                                                                       \
+    hipLaunchKernelGGL((attn_tree_kernel<RT, CG>), dim3((unsigned)nwg), dim3(THREADS), 0, stream, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, \
                        (bf16_t*)Kp, (bf16_t*)Vp, slots, pos, parents, part_o, part_ml, seg_tab, plan)
-    if (M <= 8) QT_TREE_ATTN(1, 2, 2);
-    else if (M <= 16) QT_TREE_ATTN(1, 2, 1);
-    else if (M <= 32) QT_TREE_ATTN(1, 1, 1);
-    else QT_TREE_ATTN(2, 1, 1);
+    if (M <= 8) QT_TREE_ATTN(1, 4);
+    else if (M <= 16) QT_TREE_ATTN(1, 2);
+    else if (M <= 32) QT_TREE_ATTN(1, 1);
+    else QT_TREE_ATTN(2, 1);
 #undef QT_TREE_ATTN
     QT_CHECK_LAUNCH();
     const dim3 grid((unsigned)((B * M * AH + 3) / 4));
     if (gate_rows)
-        hipLaunchKernelGGL(attn_tree_merge_kernel<true>, grid, dim3(256), 0, stream, part_o, part_ml, seg_tab, (bf16_t*)out, (const bf16_t*)gate_rows, nwg, rows, kg, plan);
+        hipLaunchKernelGGL(attn_tree_merge_kernel<true>, grid, dim3(256), 0, stream, part_o, part_ml, seg_tab, (bf16_t*)out, (const bf16_t*)gate_rows, nwg, rows, plan);
     else
-        hipLaunchKernelGGL(attn_tree_merge_kernel<false>, grid, dim3(256), 0, stream, part_o, part_ml, seg_tab, (bf16_t*)out, (const bf16_t*)nullptr, nwg, rows, kg, plan);
+        hipLaunchKernelGGL(attn_tree_merge_kernel<false>, grid, dim3(256), 0, stream, part_o, part_ml, seg_tab, (bf16_t*)out, (const bf16_t*)nullptr, nwg, rows, plan);
     QT_CHECK_LAUNCH();
     return QT_OK;
 }
@@ -456,9 +502,7 @@ int qt_internal_qkv_prep_tree(const void* qkv, const void* q_norm, const void* k
                               int table_positions, void* q, void* k, void* v, long R, int M, float eps, hipStream_t stream) __attribute__((visibility("hidden")));
 
 static long partial_bytes(int B, int M) {
-    int rows, kg;
-    shape(M, rows, kg);
-    return ((long)grid_size() + (long)B * AKV) * kg * rows * (AD + 2) * 4 + SEG_TAB_BYTES;
+    return ((long)grid_size() + (long)B * AKV) * partial_rows(M) * (AD + 2) * 4 + SEG_TAB_BYTES;
 }
 
 long qt_gqa_tree_workspace_bytes(int B, int M) {
