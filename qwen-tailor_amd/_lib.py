@@ -50,7 +50,7 @@ _SIGS = {
     "qt_rms_rows": [_vp, _vp, _vp, _i, _i, _f, _vp],
     "qt_fused_gemv_rms": [_vp, _vp, _vp, _f, _vp, _vp, _i, _i, _i, _i, _vp],
     "qt_fused_gemv": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
-    "qt_gdn_tree_step": [_vp] * 10 + [_i, _i, _i, _vp],
+    "qt_gdn_tree_step": [_vp] * 11 + [_i, _i, _i, _vp],
     "qt_gqa_tree_attn": [_vp] * 10 + [_l] + [_i] * 4 + [_vp],
     "qt_gqa_tree_layer": [_vp] * 4 + [_i] + [_vp] * 7 + [_l] + [_i] * 4 + [_f, _vp],
     "qt_tree_commit": [_vp] * 6 + [_i, _vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp],

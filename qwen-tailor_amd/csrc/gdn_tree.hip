@@ -26,13 +26,13 @@ constexpr int QK_LD = DK + 8;           // row stride (bf16) of q, k and v in LD
 constexpr float LOG_DECAY_MIN = -1e4f;  // exp of it is 0 in float; -inf would turn differences of sums into NaN
 constexpr unsigned V_MOST = (127u + 100u) << 7;      // |v| from 2^100 on, infinities and NaN, as bf16 bits
 
-// conv4 + SiLU of 8 channels of one token, as bf16 pairs (qt_common.h: conv8_silu_pairs without the table, which pays from hundreds of tokens on)
+// conv4 + SiLU of 8 channels of one token, as bf16 pairs (qt_common.h: conv8_silu_pairs without the table)
 __device__ __forceinline__ void conv8_silu(const u32x4 (&x)[4], const u32x4 (&taps)[4], uint32_t (&r)[4]) {
     float s[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const uint32_t c0 = taps[e >> 1][2 * (e & 1)], c1 = taps[e >> 1][2 * (e & 1) + 1];
         auto in = [&](int i) { return e & 1 ? hi_bf(x[i][e >> 1]) : lo_bf(x[i][e >> 1]); };
+        const uint32_t c0 = taps[e >> 1][2 * (e & 1)], c1 = taps[e >> 1][2 * (e & 1) + 1];
         s[e] = in(0) * lo_bf(c0);
         s[e] = s[e] + in(1) * hi_bf(c0);
         s[e] = s[e] + in(2) * lo_bf(c1);
@@ -48,116 +48,90 @@ __device__ __forceinline__ void conv8_silu(const u32x4 (&x)[4], const u32x4 (&ta
         r[i] = pack2_bf(lo_bf(t[i]) * lo_bf(sg), hi_bf(t[i]) * hi_bf(sg));
     }
     if (__builtin_expect(max(most.x, most.y) > (__float_as_uint(SIGMOID_FAST_MAX) >> 16), 0)) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = pack2_bf(silu_bf16(lo_bf(t[i])), silu_bf16(hi_bf(t[i])));
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) {
+            const uint32_t ti = i == 0 ? t[0] : i == 1 ? t[1] : i == 2 ? t[2] : t[3], o = pack2_bf(silu_bf16(lo_bf(ti)), silu_bf16(hi_bf(ti)));
+            r[0] = i == 0 ? o : r[0], r[1] = i == 1 ? o : r[1], r[2] = i == 2 ? o : r[2], r[3] = i == 3 ? o : r[3];
+        }
     }
 }
 
-// the row before input row i of a sequence's tokens: i >= 0 a token, -1, -2, -3 the stored window's last, middle and first row
-__device__ __forceinline__ int row_before(const int* parent_s, int i) { return i >= 0 ? parent_s[i] : max(i - 1, -3); }
-__device__ __forceinline__ const bf16_t* input_row(const bf16_t* __restrict__ proj, const bf16_t* __restrict__ window, int i) {
-    return i >= 0 ? proj + (size_t)i * PW : window + (size_t)(3 + i) * CD;
-}
-
 // One workgroup of eight wavefronts per (sequence, head); MT = 16-token tiles.  Wavefront w takes value columns 16 w .. + 15.
+//   rows   : the tokens' q, k and v input rows of this head and the stored window go to LDS directly, each once; a token's conv takes its own row and those of
+//            three ancestors from there.  (Read from memory by every token that needs them, a conv waited for its parent's index, then for four rows.)
 //   S      : lane (column n, group g) loads S[16 w + n][32 kb + 16 eh + 4 g .. + 3]: the B operand of K S^T and Q S^T when a 32-deep block is enumerated in
 //            the order (g, eh, i); k and q are stored in LDS in that order.  S = hi + lo in bf16 (off by 2^-17 of an element); k and q are bf16 already
 //   K K^T, Q K^T : bf16 MFMA, exact products; L and A in float
 //   (I + L) D = R : blocks of 16: the inverses of the diagonal blocks by forward substitution, the rest as products in float (16x16x4): an
 //            accumulator tile, register r of lane group g = row 4 g + r, is the B operand of step r for the k indices 4 g + r
-template <int MT>
+template <int MT, bool TABLE>
 __global__ __launch_bounds__(HEAD_THREADS, 2) void gdn_tree_kernel(const bf16_t* __restrict__ proj, const bf16_t* __restrict__ conv_pool,
                                                                    const bf16_t* __restrict__ cw, const float* __restrict__ A_log,
                                                                    const float* __restrict__ dt_bias, const float* __restrict__ ssm_pool,
                                                                    const int* __restrict__ slots, const int* __restrict__ pos,
-                                                                   const int* __restrict__ parents, bf16_t* __restrict__ y, int M, int n_slots) {
+                                                                   const int* __restrict__ parents, const bf16_t* __restrict__ silu_table, bf16_t* __restrict__ y, int M,
+                                                                   int n_slots) {
     constexpr int R = 16 * MT, LM_LD = R + 4;
     __shared__ __align__(16) bf16_t k_s[R * QK_LD], q_s[R * QK_LD], v_s[R * QK_LD];
-    __shared__ __align__(16) float L_s[R * LM_LD], A_s[R * LM_LD], T_s[MT * 16 * 20];
+    __shared__ __align__(1024) bf16_t raw_s[((R + 3) * 48 + 63) / 64 * 512];
+    __shared__ int up_s[R + 3];
+    // L and A, and before them the table of SiLU
+    constexpr int LA = 2 * R * LM_LD, TAB = TABLE ? SILU_TAB_SIZE / 2 : 0;
+    __shared__ __align__(1024) float la_s[LA > TAB ? LA : TAB];
+    float *const L_s = la_s, *const A_s = la_s + R * LM_LD;
+    bf16_t* const tab = reinterpret_cast<bf16_t*>(la_s);
+    __shared__ __align__(1024) bf16_t taps_s[3 * 128 * 4];
+    __shared__ __align__(16) float T_s[MT * 16 * 20];
     __shared__ double lc_s[R];
     __shared__ uint64_t anc_s[R];
     __shared__ float beta_s[R], gamma_s[R];
-    __shared__ int parent_s[R];
     __shared__ unsigned bad_s[2];
 
     const int b = blockIdx.x / HV, h = blockIdx.x % HV;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const int slot = slots[b];
     bf16_t* const yb = y + (size_t)b * M * KD + h * DV;
+    const bf16_t* const rows = proj + (size_t)b * M * PW;
+    const auto lds_of = [](void* x) { return (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(char*)x); };
+    const unsigned raw_at = lds_of(raw_s);
+    // 16-byte chunks of the rows, 48 a row, 64 a load: rows 0 .. M - 1 are the tokens', M .. M + 2 the window's, the last one first
+    auto stage = [&](int first, int end, auto row_at) {
+        for (int c0 = first + 64 * w; c0 < end; c0 += HEAD_THREADS) {
+            const int c = min(c0 + lane, end - 1), r = c / 48, k = c % 48;
+            lds_dma16_from(reinterpret_cast<const char*>(row_at(r) + (k >> 4) * KD + h * DK + 8 * (k & 15)), raw_at + 16 * (unsigned)c0);
+        }
+    };
+    const int parent = tree_parent(parents + (size_t)b * M, lane, M);            // every wavefront holds the tree, a token per lane
+    const bf16_t* const gates = rows + (size_t)min(lane, M - 1) * PW + CD + KD + h;
+    bf16_t b_raw = 0, a_raw = 0;
+    if (w == 7) b_raw = gates[0], a_raw = gates[HV];
+    const int slot = slots[b], p0 = pos[b];
+    if (w < 3) lds_dma16_from(reinterpret_cast<const char*>(cw + (size_t)(w * KD + h * DK) * 4 + 8 * lane), lds_of(taps_s) + 1024 * w);
+    if constexpr (TABLE) {
+        static_assert(SILU_TAB_SIZE == 12 * 512 + 8, "twelve whole loads, and where inputs outside the table land");
+        for (int i = w; i < 12; i += 8) lds_dma16_from(reinterpret_cast<const char*>(silu_table + 512 * i + 8 * lane), lds_of(tab) + 1024 * i);
+        if (tid == 0) *reinterpret_cast<u32x4*>(tab + SILU_TAB_HALF) = u32x4{0, 0, 0, 0};
+    }
+    // (whole loads: the tokens' rows end in the middle of one, which comes with the window)
+    const int whole = M * 48 / 64 * 64;
+    stage(0, whole, [&](int r) { return rows + (size_t)r * PW; });
+    if (tid < 2) bad_s[tid] = 0;
+    if (w == 6) {                                                // the row above each row
+        if (lane < M) up_s[lane] = parent < 0 ? M : parent;
+        if (lane < 3) up_s[M + lane] = M + min(lane + 1, 2);
+    }
+    if (w < 3)                                                   // rows past the last token: zeros
+        for (int i = 16 * M + lane; i < 16 * R; i += 64) {
+            bf16_t* const x = w == 0 ? q_s : w == 1 ? k_s : v_s;
+            *reinterpret_cast<u32x4*>(x + (i >> 4) * QK_LD + 8 * (i & 15)) = u32x4{0, 0, 0, 0};
+        }
     if ((unsigned)slot >= (unsigned)n_slots) {                   // a skipped sequence
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         for (int i = tid; i < M * 16; i += HEAD_THREADS) *reinterpret_cast<u32x4*>(yb + (size_t)(i >> 4) * KD + 8 * (i & 15)) = u32x4{0, 0, 0, 0};
         return;
     }
-    const bf16_t* const window = conv_pool + (size_t)(slot * 2 + (pos[b] & 1)) * 3 * CD;
-    const bf16_t* const rows = proj + (size_t)b * M * PW;
-    if (w == 0) {                                                // the tree and the gates, a token per lane
-        const int parent = tree_parent(parents + (size_t)b * M, lane, M);
-        const bf16_t* gates = rows + (size_t)min(lane, M - 1) * PW + CD + KD + h;
-        const float bv = bf2f(gates[0]), av = bf2f(gates[HV]);
-        const uint64_t anc = tree_ancestors(parent, lane);
-        float lg = log_decay(A_log[h], BF(av + dt_bias[h])), beta = sigmoid_bf16(bv);
-        const bool bad = lane < M && !(lg == lg && beta == beta);
-        if (bad || lane >= M) lg = 0.f, beta = 0.f;
-        const double lc = tree_path_sum(parent, (double)fmaxf(lg, LOG_DECAY_MIN), lane);
-        const uint64_t all_bad = __ballot(bad);
-        if (lane < R) {
-            parent_s[lane] = parent;
-            anc_s[lane] = anc;
-            lc_s[lane] = lc;
-            gamma_s[lane] = expf((float)lc);
-            beta_s[lane] = beta;
-        }
-        if (lane == 0) bad_s[0] = (unsigned)all_bad, bad_s[1] = (unsigned)(all_bad >> 32);
-    }
-    __syncthreads();
-
-    // conv, SiLU and norms: a row of 128 channels of one token (q, k or v) per 16 lanes
-    for (int it = tid >> 4; it < 3 * R; it += HEAD_THREADS / 16) {
-        const int part = it / R, j = it % R, ch = part * KD + h * DK + 8 * n;
-        bf16_t* const dst = (part == 0 ? q_s : part == 1 ? k_s : v_s) + j * QK_LD;
-        uint32_t u[4] = {0, 0, 0, 0};
-        if (j < M) {
-            u32x4 x[4], taps[4];
-            int i = j;
-#pragma unroll
-            for (int t = 3; t >= 0; t--) {
-                x[t] = *reinterpret_cast<const u32x4*>(input_row(rows, window, i) + ch);
-                i = row_before(parent_s, i);
-            }
-#pragma unroll
-            for (int t = 0; t < 4; t++) taps[t] = *reinterpret_cast<const u32x4*>(cw + (size_t)ch * 4 + 8 * t);
-            conv8_silu(x, taps, u);
-        }
-        if (part < 2) {
-            double sq = 0.0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const double lo = (double)lo_bf(u[e]), hi = (double)hi_bf(u[e]);
-                sq = fma(hi, hi, fma(lo, lo, sq));
-            }
-            const float r = rsqrt_rn((float)row16_sum_d(sq) / (float)DK + qk_eps());
-            const uint4 s = scale8_packed(make_uint4(u[0], u[1], u[2], u[3]), r, part == 0 ? BF(INV_SCALE * INV_SCALE) : BF(INV_SCALE));
-            u[0] = s.x, u[1] = s.y, u[2] = s.z, u[3] = s.w;
-        }
-        // A value that is not finite would reach every token through a product with zero: the token counts as bad, takes part with zeros, and its own
-        // and its descendants' outputs become NaN
-        u16x2 most = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; e++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
-        const bool bad = max(most.x, most.y) >= V_MOST;
-        const uint64_t any = __ballot(bad) >> (16 * g) & 0xffff;
-        if (any) {
-            u[0] = u[1] = u[2] = u[3] = 0;
-            if (n == 0) atomicOr(&bad_s[j >> 5], 1u << (j & 31));
-        }
-        if (part < 2) {
-            const int at = 32 * (n >> 2) + 16 * (n & 1) + 4 * ((n >> 1) & 1);
-            *reinterpret_cast<u32x2*>(dst + at) = u32x2{u[0], u[1]};
-            *reinterpret_cast<u32x2*>(dst + at + 8) = u32x2{u[2], u[3]};
-        } else {
-            *reinterpret_cast<u32x4*>(dst + 8 * n) = u32x4{u[0], u[1], u[2], u[3]};
-        }
-    }
+    const bf16_t* const window = conv_pool + (size_t)(slot * 2 + (p0 & 1)) * 3 * CD;
+    stage(whole, (M + 3) * 48, [&](int r) { return r < M ? rows + (size_t)r * PW : window + (size_t)(M + 2 - r) * CD; });
+    __builtin_amdgcn_sched_barrier(0);
     const int dv = 16 * w + n;
     f4 s[4][2];
     {
@@ -166,6 +140,81 @@ __global__ __launch_bounds__(HEAD_THREADS, 2) void gdn_tree_kernel(const bf16_t*
         for (int kb = 0; kb < 4; kb++)
 #pragma unroll
             for (int eh = 0; eh < 2; eh++) s[kb][eh] = __builtin_nontemporal_load(reinterpret_cast<const f4*>(S + 32 * kb + 16 * eh));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");             // the rows have landed; the state is behind them
+    __syncthreads();
+    // conv, SiLU and norms: items of 128 channels of one token (q, then k, then v), one per 16 lanes, four at a time per wavefront.  The last wavefront has the tree and the
+    // gates to do beside them and leaves the first round to the others: items 0 .. 27 go to wavefronts 0 .. 6, then 32 a round to all.
+    if (w == 7) {
+        float lg = log_decay(A_log[h], BF(bf2f(a_raw) + dt_bias[h])), beta = sigmoid_bf16(bf2f(b_raw));
+        const bool bad = lane < M && !(lg == lg && beta == beta);
+        if (bad || lane >= M) lg = 0.f, beta = 0.f;
+        double lc = (double)fmaxf(lg, LOG_DECAY_MIN);
+        const uint64_t anc = tree_ancestors_sum(parent, lc, lane), all_bad = __ballot(bad);
+        if (lane < R) {
+            anc_s[lane] = anc;
+            lc_s[lane] = lc;
+            gamma_s[lane] = __expf((float)lc);
+            beta_s[lane] = beta;
+        }
+        if (lane == 0) {
+            atomicOr(&bad_s[0], (unsigned)all_bad);
+            atomicOr(&bad_s[1], (unsigned)(all_bad >> 32));
+        }
+    }
+    for (int it = w < 7 ? 4 * w + g : 56 + g; __any(it < 3 * M); it = it < 28 ? 28 + 4 * w + g : it + 32) {
+        const int part = it < M ? 0 : it < 2 * M ? 1 : 2, j = min(it - part * M, M - 1);
+        const bool real = it < 3 * M;                            // (past the end a group repeats the last item and stores nothing)
+        u32x4 x[4];
+        int r = j;
+#pragma unroll
+        for (int t = 3; t >= 0; t--) {
+            x[t] = *reinterpret_cast<const u32x4*>(raw_s + r * 384 + part * 128 + 8 * n);
+            if (t > 0) r = up_s[r];
+        }
+        u32x4 taps[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) taps[e] = *reinterpret_cast<const u32x4*>(taps_s + (part * 128 + 8 * n) * 4 + 8 * e);
+        uint32_t u[4];
+        if constexpr (TABLE) {
+            auto q4 = [](const u32x4& v) { return make_uint4(v[0], v[1], v[2], v[3]); };
+            const uint4 wt[4] = {q4(taps[0]), q4(taps[1]), q4(taps[2]), q4(taps[3])};
+            conv8_silu_pairs(tab, q4(x[0]), q4(x[1]), q4(x[2]), q4(x[3]), wt, u);
+        } else {
+            conv8_silu(x, taps, u);
+        }
+        if (__any(part < 2)) {
+            double sq = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double lo = (double)lo_bf(u[e]), hi = (double)hi_bf(u[e]);
+                sq = fma(hi, hi, fma(lo, lo, sq));
+            }
+            const float rn = rsqrt_rn((float)row16_sum_d(sq) / (float)DK + qk_eps());
+            const uint4 q = scale8_packed(make_uint4(u[0], u[1], u[2], u[3]), rn, part == 0 ? BF(INV_SCALE * INV_SCALE) : BF(INV_SCALE));
+            if (part < 2) u[0] = q.x, u[1] = q.y, u[2] = q.z, u[3] = q.w;
+        }
+        // A value that is not finite would reach every token through a product with zero: the token counts as bad, takes part with zeros, and its own
+        // and its descendants' outputs become NaN
+        u16x2 most = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; e++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+        const uint64_t bad = __ballot(max(most.x, most.y) >= V_MOST);
+        if (__builtin_expect(bad != 0, 0) && (bad >> (16 * g) & 0xffff)) {
+            u[0] = u[1] = u[2] = u[3] = 0;
+            if (n == 0) atomicOr(&bad_s[j >> 5], 1u << (j & 31));
+        }
+        bf16_t* const dst = (part == 0 ? q_s : part == 1 ? k_s : v_s) + j * QK_LD;
+        if (real) {
+            if (part < 2) {
+                const int at = 32 * (n >> 2) + 16 * (n & 1) + 4 * ((n >> 1) & 1);
+                *reinterpret_cast<u32x2*>(dst + at) = u32x2{u[0], u[1]};
+                *reinterpret_cast<u32x2*>(dst + at + 8) = u32x2{u[2], u[3]};
+            } else {
+                *reinterpret_cast<u32x4*>(dst + 8 * n) = u32x4{u[0], u[1], u[2], u[3]};
+            }
+        }
     }
     __syncthreads();
 
@@ -184,7 +233,7 @@ __global__ __launch_bounds__(HEAD_THREADS, 2) void gdn_tree_kernel(const bf16_t*
         for (int r = 0; r < 4; r++) {
             const int i = 16 * I + 4 * g + r;
             const bool on = (anc_s[i] >> j & 1) && (is_a || i != j);
-            const float G = on ? expf((float)(lc_s[i] - lc_s[j])) : 0.f;
+            const float G = on ? __expf((float)(lc_s[i] - lc_s[j])) : 0.f;
             (is_a ? A_s : L_s)[i * LM_LD + j] = on ? acc[r] * (is_a ? G : -beta_s[i] * G) : 0.f;
         }
     }
@@ -407,21 +456,26 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 extern "C" {
 
 int qt_gdn_tree_step(const void* proj, const void* conv_pool, const void* conv_w, const float* A_log, const float* dt_bias, const float* ssm_pool,
-                     const int32_t* slots, const int32_t* pos, const int32_t* parents, void* y, int B, int M, int n_slots, hipStream_t stream) {
+                     const int32_t* slots, const int32_t* pos, const int32_t* parents, const void* silu_table, void* y, int B, int M, int n_slots,
+                     hipStream_t stream) {
     if (B < 0 || n_slots < 1 || B > (1 << 26)) return QT_ERR_DIM;
     if (M < 1 || M > TREE_MAX) return QT_ERR_UNSUPPORTED;
     if (B == 0) return QT_OK;
     if (!proj || !conv_pool || !conv_w || !A_log || !dt_bias || !ssm_pool || !slots || !pos || !parents || !y) return QT_ERR_NULL;
-    for (const void* p : {proj, conv_pool, conv_w, (const void*)ssm_pool, (const void*)y})
+    for (const void* p : {proj, conv_pool, conv_w, (const void*)ssm_pool, silu_table, (const void*)y})
         if (!aligned16(p)) return QT_ERR_ALIGN;
-#define QT_TREE(MT)                                                                                                                              \
-    hipLaunchKernelGGL((gdn_tree_kernel<MT>), dim3((unsigned)B * HV), dim3(HEAD_THREADS), 0, stream, (const bf16_t*)proj, (const bf16_t*)conv_pool, \
-                       (const bf16_t*)conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, (bf16_t*)y, M, n_slots)
-    switch ((M + 15) / 16) {
-        case 1: QT_TREE(1); break;
-        case 2: QT_TREE(2); break;
-        case 3: QT_TREE(3); break;
-        default: QT_TREE(4); break;
+    // SiLU from the table from 17 tokens on: below it is evaluated by fewer wavefronts than the table takes to arrive
+#define QT_TREE(MT, TABLE)                                                                                                                            \
+    hipLaunchKernelGGL((gdn_tree_kernel<MT, TABLE>), dim3((unsigned)B * HV), dim3(HEAD_THREADS), 0, stream, (const bf16_t*)proj,                       \
+                       (const bf16_t*)conv_pool, (const bf16_t*)conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, (const bf16_t*)silu_table, (bf16_t*)y, \
+                       M, n_slots)
+    switch ((M + 15) / 16 * (silu_table ? 2 : 1)) {
+        case 2: if (M <= 16) QT_TREE(1, false); else QT_TREE(2, false); break;
+        case 1: QT_TREE(1, false); break;
+        case 3: QT_TREE(3, false); break;
+        case 4: if (silu_table) QT_TREE(2, true); else QT_TREE(4, false); break;
+        case 6: QT_TREE(3, true); break;
+        default: QT_TREE(4, true); break;
     }
 #undef QT_TREE
     QT_CHECK_LAUNCH();

@@ -941,10 +941,12 @@ PyObject* deltanet_bt(PyObject* const* a) {
     const OnDevice on(proj);
     const Tensor A = f32(a[3], "A_log", HV), dtb = f32(a[4], "dt_bias", HV);
     on(conv, "conv_pool"), on(w, "conv_w"), on(A, "A_log"), on(dtb, "dt_bias"), on(ssm, "ssm_pool"), on(slots, "slots"), on(pos, "pos"), on(parents, "parents");
+    const Tensor silu = M > 16 && B > 0 ? silu_table(proj) : Tensor();
     return wrap(unlocked([&] {
         Tensor y = empty({B * M, HV * DV}, BF16, proj);
         check(qt_gdn_tree_step(proj.data_ptr(), conv.data_ptr(), w.data_ptr(), A.data_ptr<float>(), dtb.data_ptr<float>(), ssm.data_ptr<float>(),
-                               slots.data_ptr<int>(), pos.data_ptr<int>(), parents.data_ptr<int>(), y.data_ptr(), dim32(B), dim32(M), dim32(n_slots), stream()),
+                               slots.data_ptr<int>(), pos.data_ptr<int>(), parents.data_ptr<int>(), silu.defined() ? silu.data_ptr() : nullptr, y.data_ptr(), dim32(B), dim32(M),
+                               dim32(n_slots), stream()),
               "qt_gdn_tree_step");
         return y;
     }));

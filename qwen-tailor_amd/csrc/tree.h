@@ -31,17 +31,19 @@ __device__ __forceinline__ uint64_t tree_ancestors(int parent, int lane) {
     }
     return seen;
 }
-// sum of v over the lane's token and its ancestors
-__device__ __forceinline__ double tree_path_sum(int parent, double v, int lane) {
+// the same, and v becomes the sum of v over the lane's token and its ancestors
+__device__ __forceinline__ uint64_t tree_ancestors_sum(int parent, double& v, int lane) {
+    uint64_t seen = 1ull << lane | (parent >= 0 ? 1ull << parent : 0);
     int a = parent;
 #pragma unroll
     for (int i = 0; i < 6; i++) {
         const int from = a < 0 ? lane : a;
-        const double s = __hiloint2double(__shfl(__double2hiint(v), from), __shfl(__double2loint(v), from));
+        const uint64_t s = shfl64(seen, from);
+        const double d = __hiloint2double(__shfl(__double2hiint(v), from), __shfl(__double2loint(v), from));
         const int up = __shfl(a, from);
-        if (a >= 0) v += s, a = up;
+        if (a >= 0) seen |= s, v += d, a = up;
     }
-    return v;
+    return seen;
 }
 
 }  // namespace qt

@@ -22,11 +22,12 @@ def test_error_codes():
     lib = qt._lib.lib()
     z, p, odd = ctypes.c_void_p(0), ctypes.c_void_p(16), ctypes.c_void_p(8)
     step = lambda *a: lib.qt_gdn_tree_step(*a)  # noqa: E731
-    assert step(p, p, p, p, p, p, p, p, z, p, 1, 4, 1, z) == -3
-    assert step(p, p, p, p, p, p, p, p, p, p, 1, 65, 1, z) == -4 and step(p, p, p, p, p, p, p, p, p, p, 1, 0, 1, z) == -4
-    assert step(p, p, p, p, p, p, p, p, p, p, -1, 4, 1, z) == -1 and step(p, p, p, p, p, p, p, p, p, p, 1, 4, 0, z) == -1
-    assert step(odd, p, p, p, p, p, p, p, p, p, 1, 4, 1, z) == -2
-    assert step(p, p, p, p, p, p, p, p, p, p, 0, 4, 1, z) == 0                       # nothing to do: no launch
+    assert step(p, p, p, p, p, p, p, p, z, p, p, 1, 4, 1, z) == -3
+    assert step(p, p, p, p, p, p, p, p, p, z, p, 1, 65, 1, z) == -4 and step(p, p, p, p, p, p, p, p, p, z, p, 1, 0, 1, z) == -4
+    assert step(p, p, p, p, p, p, p, p, p, z, p, -1, 4, 1, z) == -1 and step(p, p, p, p, p, p, p, p, p, z, p, 1, 4, 0, z) == -1
+    assert step(p, p, p, p, p, p, p, p, p, odd, p, 1, 4, 1, z) == -2
+    assert step(odd, p, p, p, p, p, p, p, p, z, p, 1, 4, 1, z) == -2
+    assert step(p, p, p, p, p, p, p, p, p, z, p, 0, 4, 1, z) == 0                       # nothing to do: no launch
     need = lib.qt_gqa_tree_workspace_bytes(2, 16)
     assert lib.qt_gqa_tree_workspace_bytes(1025, 4) == -1 and lib.qt_gqa_tree_workspace_bytes(1, 65) == -1 and lib.qt_gqa_tree_layer_workspace_bytes(1, 0) == -1
     assert lib.qt_gqa_tree_layer_workspace_bytes(2, 16) >= need + 2 * 16 * 12 * 256 * 2
