@@ -277,7 +277,8 @@ int qt_gqa_tree_layer(const void* qkv, const void* q_norm, const void* k_norm, c
  * count [B] how many of them (<= 0: nothing happens; more than D count as D).  For each of the n_gdn recurrent layers (tables of
  * device pointers in host memory: proj [B*M,8224], conv_pool, conv_w, A_log, dt_bias, ssm_pool) the state advances in place through those tokens with the
  * bits of as many calls of qt_gdn_decode_step, and the new window goes to conv buffer (pos + count) & 1.  For each of the n_kv K / V pools
- * [n_slots,2,Lmax,256] rows pos + path[j] move to pos + j.  The sequence then holds pos + count tokens.  With K / V pools a sequence with pos < 0 or
+ * [n_slots,2,Lmax,256] rows pos + path[j] move to pos + j (all read before the first is written; a path entry that is no token counts as
+ * token 0).  The sequence then holds pos + count tokens.  With K / V pools a sequence with pos < 0 or
  * pos + M > Lmax is skipped, as by the attention. */
 int qt_tree_commit(const void* const* proj, void* const* conv_pool, const void* const* conv_w, const float* const* A_log, const float* const* dt_bias,
                    float* const* ssm_pool, int n_gdn, void* const* kv_pool, int n_kv, const int32_t* slots, const int32_t* pos, const int32_t* path,

@@ -10,6 +10,8 @@
 //     d_i + sum over strict ancestors j of beta_i G_ij (k_i . k_j) d_j = beta_i (v_i - gamma_i S k_i)            (I + L) D = R
 //     y_i = gamma_i S q_i + sum over ancestors and itself of G_ij (q_i . k_j) d_j                                Y = gamma Q S^T + A D
 // A parent comes before its children, so I + L is lower triangular whatever the tree looks like: a token that is no ancestor leaves a zero.
+#include <algorithm>
+
 #include "tree.h"
 
 using namespace qt;
@@ -346,28 +348,41 @@ __device__ __forceinline__ bool takes_part(int slot, int p0, int M, int n_slots,
 // The tokens path[0 .. count - 1] of one (layer, sequence, head), through the recurrence of a decode step: the same bits.  The state stays in
 // registers from its load to its store.  The conv window of a sequence lies in buffer pos & 1 and goes to buffer (pos + count) & 1, which for an
 // even count is the same: all of this head's channels are read before the first is written, and no other workgroup reads them.
-__global__ __launch_bounds__(256, 3) void gdn_commit_kernel(const GdnLayers layers, const int* __restrict__ slots, const int* __restrict__ pos,
-                                                            const int* __restrict__ path, const int* __restrict__ count, int B, int M, int D,
-                                                            int n_slots, int Lmax) {
-    __shared__ double red[2];
-    __shared__ __align__(16) float k_s[DK];
-    __shared__ float v_s[DV], gb_s[2];
-    const int h = blockIdx.x % HV, b = blockIdx.x / HV % B, layer = blockIdx.x / HV / B;
+// Tokens are prepared four at a time (rows asked for a group ahead, conv, norms and gates of the four side by side, two barriers): the first group while the
+// state is on its way.  One at a time, a single sequence waited for memory at every token.
+constexpr int GROUP = 4;
+__device__ __forceinline__ void gdn_commit(const GdnLayers& layers, int block, const int* __restrict__ slots, const int* __restrict__ pos, const int* __restrict__ path,
+                                           const int* __restrict__ count, int B, int M, int D, int n_slots, int Lmax) {
+    __shared__ double red[GROUP][2];
+    __shared__ __align__(16) float k_s[GROUP][DK];
+    __shared__ float v_s[GROUP][DV], gb_s[2 * GROUP];
+    const int h = block % HV, b = block / HV % B, layer = block / HV / B;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane >> 4, c = lane & 15;
+    const int token = lane < D ? path_token(path + (size_t)b * D, lane, M) : 0;           // entry j of the path in lane j
     const int slot = slots[b], p0 = pos[b], cnt = min(count[b], D);
     if (!takes_part(slot, p0, M, n_slots, Lmax) || cnt <= 0) return;
     const bf16_t* const proj = layers.proj[layer] + (size_t)b * M * PW;
-    const bf16_t* const cw = layers.cw[layer];
     const bf16_t* const window = layers.conv[layer] + (size_t)(slot * 2 + (p0 & 1)) * 3 * CD;
     bf16_t* const window_out = layers.conv[layer] + (size_t)(slot * 2 + ((p0 + cnt) & 1)) * 3 * CD;
-    const int* const mine = path + (size_t)b * D;
     // threads 0 .. 127 a k channel, 128 .. 255 a v channel; q only moves through the window (threads 0 .. 127)
     const int ch = (tid < 128 ? KD : 2 * KD) + h * DK + (tid & 127), ch_q = h * DK + (tid & 127);
-    const uint2 taps = *reinterpret_cast<const uint2*>(cw + (size_t)ch * 4);
+    unsigned now[GROUP], now_q[GROUP];
+    bf16_t gate_raw = 0;
+    auto fetch = [&](int j0) {                                   // (past the path's end: its last token again)
+#pragma unroll
+        for (int t = 0; t < GROUP; t++) {
+            const bf16_t* const row = proj + (size_t)__builtin_amdgcn_readlane(token, min(j0 + t, cnt - 1)) * PW;
+            now[t] = row[ch], now_q[t] = row[ch_q];
+        }
+        if (w == 3) gate_raw = proj[(size_t)__shfl(token, min(j0 + (lane >> 1 & 3), cnt - 1)) * PW + CD + KD + (lane & 1) * HV + h];
+    };
+    const uint2 taps = *reinterpret_cast<const uint2*>(layers.cw[layer] + (size_t)ch * 4);
     const float gA = layers.A_log[layer][h], gdt = layers.dt_bias[layer][h];
     unsigned x[3], xq[3];
 #pragma unroll
     for (int i = 0; i < 3; i++) x[i] = window[i * CD + ch], xq[i] = window[i * CD + ch_q];
+    fetch(0);
+    __builtin_amdgcn_sched_barrier(0);
     f4 s[8][2];
     f4* const S = reinterpret_cast<f4*>(layers.ssm[layer] + ((size_t)slot * HV + h) * DV * DK);
 #pragma unroll
@@ -376,41 +391,57 @@ __global__ __launch_bounds__(256, 3) void gdn_commit_kernel(const GdnLayers laye
         s[i][0] = __builtin_nontemporal_load(S + row * (DK / 4) + c);
         s[i][1] = __builtin_nontemporal_load(S + row * (DK / 4) + 16 + c);
     }
-    for (int j = 0; j < cnt; j++) {
-        const bf16_t* row = proj + (size_t)path_token(mine, j, M) * PW;
-        const unsigned now = row[ch], now_q = row[ch_q];
-        const float u = conv_silu(bf2f((bf16_t)x[0]), bf2f((bf16_t)x[1]), bf2f((bf16_t)x[2]), bf2f((bf16_t)now), taps);
-        x[0] = x[1], x[1] = x[2], x[2] = now;
-        xq[0] = xq[1], xq[1] = xq[2], xq[2] = now_q;
+    __builtin_amdgcn_sched_barrier(0);
+    for (int j0 = 0; j0 < cnt; j0 += GROUP) {
+        float u[GROUP];
+#pragma unroll
+        for (int t = 0; t < GROUP; t++) {
+            u[t] = conv_silu(bf2f((bf16_t)x[0]), bf2f((bf16_t)x[1]), bf2f((bf16_t)x[2]), bf2f((bf16_t)now[t]), taps);
+            if (j0 + t < cnt) {
+                x[0] = x[1], x[1] = x[2], x[2] = now[t];
+                xq[0] = xq[1], xq[1] = xq[2], xq[2] = now_q[t];
+            }
+        }
         if (w < 2) {
-            const double tot = wave_sum_d((double)u * (double)u);
-            if (lane == 0) red[w] = tot;
+#pragma unroll
+            for (int t = 0; t < GROUP; t++) {
+                const double tot = wave_sum_d((double)u[t] * (double)u[t]);
+                if (lane == 0) red[t][w] = tot;
+            }
         } else {
-            v_s[tid - 128] = u;
+#pragma unroll
+            for (int t = 0; t < GROUP; t++) v_s[t][tid - 128] = u[t];
         }
         if (w == 3) {
-            const float gv = bf2f(row[CD + KD + (lane == 1 ? HV : 0) + h]);
-            const float gate = lane == 1 ? decay_gate(gA, BF(gv + gdt)) : sigmoid_bf16(gv);
-            if (lane < 2) gb_s[lane] = gate;                     // beta, g
+            const float gv = bf2f(gate_raw), gate = lane & 1 ? decay_gate(gA, BF(gv + gdt)) : sigmoid_bf16(gv);
+            if (lane < 2 * GROUP) gb_s[lane] = gate;             // beta, g of each token
         }
         __syncthreads();
         if (w < 2) {
-            const float r = rsqrt_rn((float)(red[0] + red[1]) / (float)DK + qk_eps());
-            k_s[tid] = BF(BF(u * r) * BF(INV_SCALE));
+#pragma unroll
+            for (int t = 0; t < GROUP; t++) {
+                const float r = rsqrt_rn((float)(red[t][0] + red[t][1]) / (float)DK + qk_eps());
+                k_s[t][tid] = BF(BF(u[t] * r) * BF(INV_SCALE));
+            }
         }
         __syncthreads();
-        float k8[8];
-        {
-            const float4 a = reinterpret_cast<const float4*>(k_s)[c], e = reinterpret_cast<const float4*>(k_s)[16 + c];
-            k8[0] = a.x, k8[1] = a.y, k8[2] = a.z, k8[3] = a.w, k8[4] = e.x, k8[5] = e.y, k8[6] = e.z, k8[7] = e.w;
-        }
-        const float beta = gb_s[0], gg = gb_s[1];
+        if (j0 + GROUP < cnt) fetch(j0 + GROUP);
+        const int here = min(GROUP, cnt - j0);
+#pragma unroll 1
+        for (int t = 0; t < here; t++) {
+            float k8[8];
+            {
+                const float4 a = reinterpret_cast<const float4*>(k_s[t])[c], e = reinterpret_cast<const float4*>(k_s[t])[16 + c];
+                k8[0] = a.x, k8[1] = a.y, k8[2] = a.z, k8[3] = a.w, k8[4] = e.x, k8[5] = e.y, k8[6] = e.z, k8[7] = e.w;
+            }
+            const float beta = gb_s[2 * t], gg = gb_s[2 * t + 1];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float sv[8] = {s[i][0].x, s[i][0].y, s[i][0].z, s[i][0].w, s[i][1].x, s[i][1].y, s[i][1].z, s[i][1].w};
-            gdn_row_step(sv, k8, k8, v_s[i * 16 + w * 4 + grp], gg, beta, 0.f);
-            s[i][0] = f4{sv[0], sv[1], sv[2], sv[3]};
-            s[i][1] = f4{sv[4], sv[5], sv[6], sv[7]};
+            for (int i = 0; i < 8; i++) {
+                float sv[8] = {s[i][0].x, s[i][0].y, s[i][0].z, s[i][0].w, s[i][1].x, s[i][1].y, s[i][1].z, s[i][1].w};
+                gdn_row_step(sv, k8, k8, v_s[t][i * 16 + w * 4 + grp], gg, beta, 0.f);
+                s[i][0] = f4{sv[0], sv[1], sv[2], sv[3]};
+                s[i][1] = f4{sv[4], sv[5], sv[6], sv[7]};
+            }
         }
         __syncthreads();
     }
@@ -427,26 +458,36 @@ __global__ __launch_bounds__(256, 3) void gdn_commit_kernel(const GdnLayers laye
     }
 }
 
-// K / V rows pos + path[j] -> pos + j of one (pool, sequence, head), eight rows of 512 bytes at a time.  A path goes down a tree, so path[j] >= j grows with
-// j: no row is overwritten before it has been read.
-__global__ __launch_bounds__(256) void kv_commit_kernel(const KvLayers layers, const int* __restrict__ slots, const int* __restrict__ pos,
-                                                        const int* __restrict__ path, const int* __restrict__ count, int B, int M, int D, int n_slots,
-                                                        int Lmax) {
-    const int head = blockIdx.x % AKV, b = blockIdx.x / AKV % B, pool = blockIdx.x / AKV / B;
+// K / V rows pos + path[j] -> pos + j of one (pool, sequence, head): eight rows of 512 bytes at a time, all read before the first is written
+__device__ __forceinline__ void kv_commit(const KvLayers& layers, int block, const int* __restrict__ slots, const int* __restrict__ pos, const int* __restrict__ path,
+                                          const int* __restrict__ count, int B, int M, int D, int n_slots, int Lmax) {
+    const int head = block % AKV, b = block / AKV % B, pool = block / AKV / B;
+    const int lane = threadIdx.x & 63, j0 = threadIdx.x >> 5, c = threadIdx.x & 31;
+    const int token = lane < D ? path_token(path + (size_t)b * D, lane, M) : 0;
     const int slot = slots[b], p0 = pos[b], cnt = min(count[b], D);
     if (!takes_part(slot, p0, M, n_slots, Lmax)) return;
-    u32x4* const base = reinterpret_cast<u32x4*>(layers.pool[pool] + (((size_t)slot * AKV + head) * Lmax + p0) * AD);
-    for (int j0 = 0; j0 < cnt; j0 += 8) {
-        const int j = j0 + (threadIdx.x >> 5), c = threadIdx.x & 31;
-        int from = j;
-        u32x4 v = {0, 0, 0, 0};
-        if (j < cnt) {
-            from = path_token(path + (size_t)b * D, j, M);
-            if (from != j) v = base[(size_t)from * (AD / 8) + c];
-        }
-        __syncthreads();
-        if (from != j) base[(size_t)j * (AD / 8) + c] = v;
+    u32x4* const base = reinterpret_cast<u32x4*>(layers.pool[pool] + (((size_t)slot * AKV + head) * Lmax + p0) * AD) + c;
+    u32x4 v[TREE_MAX / 8];
+#pragma unroll
+    for (int i = 0; i < TREE_MAX / 8; i++) {
+        const int from = __shfl(token, 8 * i + j0);
+        v[i] = u32x4{0, 0, 0, 0};
+        if (8 * i < cnt && 8 * i + j0 < cnt) v[i] = base[(size_t)from * (AD / 8)];
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TREE_MAX / 8; i++)
+        if (8 * i + j0 < cnt) base[(size_t)(8 * i + j0) * (AD / 8)] = v[i];
+}
+
+// both kinds in one launch (a second one cost a single sequence 2 us); the short ones of the K / V rows last
+__global__ __launch_bounds__(256, 2) void commit_kernel(const GdnLayers gdn, const KvLayers kv, int n_gdn, const int* __restrict__ slots, const int* __restrict__ pos,
+                                                        const int* __restrict__ path, const int* __restrict__ count, int B, int M, int D, int n_slots, int Lmax) {
+    const int gdn_blocks = n_gdn * B * HV, block = blockIdx.x;
+    if (block < gdn_blocks)
+        gdn_commit(gdn, block, slots, pos, path, count, B, M, D, n_slots, Lmax);
+    else
+        kv_commit(kv, block - gdn_blocks, slots, pos, path, count, B, M, D, n_slots, Lmax);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -469,14 +510,13 @@ int qt_gdn_tree_step(const void* proj, const void* conv_pool, const void* conv_w
     hipLaunchKernelGGL((gdn_tree_kernel<MT, TABLE>), dim3((unsigned)B * HV), dim3(HEAD_THREADS), 0, stream, (const bf16_t*)proj,                       \
                        (const bf16_t*)conv_pool, (const bf16_t*)conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, (const bf16_t*)silu_table, (bf16_t*)y, \
                        M, n_slots)
-    switch ((M + 15) / 16 * (silu_table ? 2 : 1)) {
-        case 2: if (M <= 16) QT_TREE(1, false); else QT_TREE(2, false); break;
-        case 1: QT_TREE(1, false); break;
-        case 3: QT_TREE(3, false); break;
-        case 4: if (silu_table) QT_TREE(2, true); else QT_TREE(4, false); break;
-        case 6: QT_TREE(3, true); break;
-        default: QT_TREE(4, true); break;
-    }
+    if (M <= 16) QT_TREE(1, false);
+    else if (M <= 32 && silu_table) QT_TREE(2, true);
+    else if (M <= 32) QT_TREE(2, false);
+    else if (M <= 48 && silu_table) QT_TREE(3, true);
+    else if (M <= 48) QT_TREE(3, false);
+    else if (silu_table) QT_TREE(4, true);
+    else QT_TREE(4, false);
 #undef QT_TREE
     QT_CHECK_LAUNCH();
     return QT_OK;
@@ -501,26 +541,21 @@ int qt_tree_commit(const void* const* proj, void* const* conv_pool, const void* 
         if (!kv_pool[i]) return QT_ERR_NULL;
         if (!aligned16(kv_pool[i])) return QT_ERR_ALIGN;
     }
-    for (int l0 = 0; l0 < n_gdn; l0 += COMMIT_LAYERS) {
-        GdnLayers t = {};
-        const int nl = n_gdn - l0 < COMMIT_LAYERS ? n_gdn - l0 : COMMIT_LAYERS;
-        for (int i = 0; i < nl; i++) {
-            t.proj[i] = (const bf16_t*)proj[l0 + i];
-            t.conv[i] = (bf16_t*)conv_pool[l0 + i];
-            t.cw[i] = (const bf16_t*)conv_w[l0 + i];
-            t.A_log[i] = A_log[l0 + i];
-            t.dt_bias[i] = dt_bias[l0 + i];
-            t.ssm[i] = ssm_pool[l0 + i];
+    for (int g0 = 0, k0 = 0; g0 < n_gdn || k0 < n_kv; g0 += COMMIT_LAYERS, k0 += 2 * COMMIT_LAYERS) {
+        GdnLayers gdn = {};
+        KvLayers kv = {};
+        const int ng = std::max(0, std::min(n_gdn - g0, COMMIT_LAYERS)), nk = std::max(0, std::min(n_kv - k0, 2 * COMMIT_LAYERS));
+        for (int i = 0; i < ng; i++) {
+            gdn.proj[i] = (const bf16_t*)proj[g0 + i];
+            gdn.conv[i] = (bf16_t*)conv_pool[g0 + i];
+            gdn.cw[i] = (const bf16_t*)conv_w[g0 + i];
+            gdn.A_log[i] = A_log[g0 + i];
+            gdn.dt_bias[i] = dt_bias[g0 + i];
+            gdn.ssm[i] = ssm_pool[g0 + i];
         }
-        hipLaunchKernelGGL(gdn_commit_kernel, dim3((unsigned)nl * B * HV), dim3(256), 0, stream, t, slots, pos, path, count, B, M, D, n_slots,
+        for (int i = 0; i < nk; i++) kv.pool[i] = (bf16_t*)kv_pool[k0 + i];
+        hipLaunchKernelGGL(commit_kernel, dim3((unsigned)B * (ng * HV + nk * AKV)), dim3(256), 0, stream, gdn, kv, ng, slots, pos, path, count, B, M, D, n_slots,
                            n_kv > 0 ? Lmax : 0);
-        QT_CHECK_LAUNCH();
-    }
-    for (int l0 = 0; l0 < n_kv; l0 += 2 * COMMIT_LAYERS) {
-        KvLayers t = {};
-        const int nl = n_kv - l0 < 2 * COMMIT_LAYERS ? n_kv - l0 : 2 * COMMIT_LAYERS;
-        for (int i = 0; i < nl; i++) t.pool[i] = (bf16_t*)kv_pool[l0 + i];
-        hipLaunchKernelGGL(kv_commit_kernel, dim3((unsigned)nl * B * AKV), dim3(256), 0, stream, t, slots, pos, path, count, B, M, D, n_slots, Lmax);
         QT_CHECK_LAUNCH();
     }
     return QT_OK;

@@ -320,6 +320,18 @@ def test_gdn_step_skips(dev):
     check_tensors_equal("the others", y[[0, 2]], gdn_run(c, dev).reshape(4, -1)[[0, 2]])
 
 
+@pytest.mark.parametrize("M", [16, 17, 33, 64])
+def test_gdn_step_without_the_table(dev, M):
+    """the C entry takes a null table of SiLU: it evaluates the function, the same bits"""
+    import qwen_tailor_amd as qt
+    c = gdn_case(300 + M, 2, M, "random", scale=3.0)
+    want = gdn_run(c, dev)
+    t = [to_dev(c["proj"], dev, BF16), to_dev(c["conv"], dev, BF16), to_dev(c["cw"], dev, BF16)] + [to_dev(c[n], dev) for n in ("A_log", "dtb", "ssm", "slots", "pos", "parents")]
+    y = torch.empty_like(want)
+    qt._lib.call("qt_gdn_tree_step", *[qt._lib.ptr(x) for x in t], None, qt._lib.ptr(y), 2, M, 3, qt._lib.stream())
+    check_tensors_equal("y", y, want)
+
+
 # ---- the commit ----------------------------------------------------------------------------------------------------------
 
 class PoolSet:
@@ -402,6 +414,24 @@ def test_commit_skips(dev):
     qt.batch_tree.commit(b, [proj], [p[0]], [p[1]], [p[2]], i([0, 1, 2, 3, 4]), i([3] * 5), i([[0, 0, 0]] * B), i([3] * 5))
     for name in ("conv", "ssm"):
         check_tensors_equal(name, getattr(a, name)[0], getattr(b, name)[0])
+
+
+def test_commit_gathers_whatever_the_path_says(dev):
+    """K / V rows of a path that goes down no tree (backwards, repeated): every row as it was before the call"""
+    import qwen_tailor_amd as qt
+    gen = torch.Generator(dev).manual_seed(2)
+    B, M, D, Lmax = 2, 64, 64, 100
+    P = PoolSet(gen, 0, 2, 3, Lmax, dev)
+    path = torch.stack([torch.arange(63, -1, -1), torch.arange(64) // 5 * 3]).to(torch.int32).to(dev)
+    slots, pos, count = (torch.tensor(a, dtype=torch.int32, device=dev) for a in ([2, 0], [36, 5], [64, 41]))
+    got = P.clone()
+    qt.batch_tree.commit(got, [], [], [], [], slots, pos, path, count, M=M)
+    for name in ("K", "V"):
+        for a, old in zip(getattr(got, name), getattr(P, name)):
+            want = old.clone()
+            for b, (s, p, n) in enumerate([(2, 36, 64), (0, 5, 41)]):
+                want[s, :, p:p + n] = old[s][:, (p + path[b, :n]).long()]
+            check_tensors_equal(name, a, want)
 
 
 # ---- a round ------------------------------------------------------------------------------------------------------------
