@@ -32,12 +32,23 @@ constexpr float SCALE_LOG2E = 0.0625f * 1.44269504088896f;                     /
 constexpr float NEG = -3.0e38f;
 constexpr int MAX_SEG = 2048, MAX_GRID = 1024;
 
+// the larger of two floats in one instruction (the compiler makes three of fmaxf behind a lane exchange, to quiet signalling NaN)
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+    unsigned r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
 __device__ __forceinline__ float max_over_groups(float x) {      // over the lanes n, n + 16, n + 32, n + 48
     const unsigned xi = __float_as_uint(x);
     const auto a = __builtin_amdgcn_permlane32_swap(xi, xi, false, false);
-    const unsigned mi = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const unsigned mi = larger(a[0], a[1]);
     const auto b = __builtin_amdgcn_permlane16_swap(mi, mi, false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    return __uint_as_float(larger(b[0], b[1]));
+}
+// c + the two bf16 of a word, products and sum in float
+__device__ __forceinline__ float pair_sum(unsigned w, float c) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
 }
 __device__ __forceinline__ float sum_over_groups(float x) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -56,8 +67,8 @@ __device__ __forceinline__ int segment_tiles(const Plan& p, int slot, int p0) {
 }
 __device__ __forceinline__ int tiles_per_wg(int total, int nwg, int min_tiles) { return max(min_tiles, (total + nwg - 1) / nwg); }
 
-// a copy the compiler cannot see through: what is derived from it is computed again where it is used (the lane-dependent addresses of the tile loop would
-// live in about 50 registers across it)
+// a copy the compiler cannot see through: what is derived from it is computed again where it is used (with two row tiles a wavefront the lane-dependent
+// addresses of the tile loop would live in registers that it does not have)
 __device__ __forceinline__ int opaque(int v) {
     asm volatile("" : "+v"(v));
     return v;
@@ -102,6 +113,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
     // P as two bf16 terms (off by 2^-17) while the launch is bound by the cache's bytes.  With two row tiles a wavefront the second product would cost a half
     // more MFMA time: P is rounded once (2^-9 of each weight, the sum is taken of the rounded ones), less than the output's own rounding.
     constexpr bool SPLIT = RT == 1;
+    constexpr int DEPTH = RT == 1 ? 6 : 4;                       // fragments on their way from LDS
     __shared__ __align__(1024) unsigned char tile_s[BUFS * 2 * TILE_BYTES];
     __shared__ int seg_start[MAX_SEG + 1];
     __shared__ uint64_t seen_s[TREE_MAX];                        // bit i of entry j: token j sees new key i
@@ -185,7 +197,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         const int key0 = (is_new ? t - pool_tiles : t) * KT, left = (is_new ? M : v.p0) - key0;
         const size_t at = is_new ? new_rows(v) + (size_t)key0 * (AKV * AD) : pool_rows(v) + (size_t)key0 * AD;
         const bf16_t *ks = (is_new ? k_new : Kp) + at, *vs = (is_new ? v_new : Vp) + at;
-        const int ln = opaque(lane);
+        const int ln = RT > 1 ? opaque(lane) : lane;
 #pragma unroll
         for (int i = 0; i < PAIRS; i++) {
             int r = 2 * (w + WAVES * i) + (ln >> 5);
@@ -219,8 +231,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         const int pool_tiles = (v.p0 + KT - 1) / KT;
         const bool has_new = v.t1 > pool_tiles;
         if (has_new && w == 0) {
-            if (lane < 2) bad_s[lane] = 0;
-            seen_s[lane] = tree_ancestors(tree_parent(parents + (size_t)(v.sg / AKV) * M, lane, M), lane);
+            const int ln = opaque(lane);
+            if (ln < 2) bad_s[ln] = 0;
+            seen_s[ln] = tree_ancestors(tree_parent(parents + (size_t)(v.sg / AKV) * M, ln, M), ln);
         }
         // q is waited for here: in the tile loop the compiler would wait for its loads in every turn, and for the tiles in flight with them
 #pragma unroll
@@ -262,22 +275,50 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                 }
                 __syncthreads();
             }
-            const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+            const int ln = RT > 1 ? opaque(lane) : lane, n = ln & 15, g = ln >> 4;
+            // The fragments of K, then of V, come out of LDS DEPTH steps ahead of their products: what is asked for only just before stands in the way of all that follows.
+            // A operand: lane (key n, group g) holds k[key][32 kb + 8 g .. + 8].  V by the transposing load: lane (n, g) points at key 4 g + n / 4, columns 4 (n % 4) ..
+            // + 3 of the block, and receives keys 4 g .. + 3 of column n.  Two of them are the A operand when the 32 keys are enumerated as 16 (e >> 2) + 4 g +
+            // (e & 3), in which order the lane holds its probabilities.
             f32x4 s[RT][KT / 16];
 #pragma unroll
-            for (int u = 0; u < KT / 16; u++) {
-                if (RT > 1) __builtin_amdgcn_sched_barrier(0);
-                const unsigned at = (16 * u + n) * ROW_BYTES + ((g ^ n) << 4);     // A operand: lane (key n, group g) holds k[key][32 kb + 8 g .. + 8]
+            for (int t = 0; t < RT; t++)
 #pragma unroll
-                for (int t = 0; t < RT; t++) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int u = 0; u < KT / 16; u++) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const unsigned kat = n * ROW_BYTES + ((g ^ n) << 4);
+            auto k_frag = [&](int x) {                           // step x: block kb = x / 2 of keys 16 (x % 2) .. + 15
+                return *reinterpret_cast<const u32x4*>(kt + (kat ^ ((x >> 1 & 3) << 6)) + (x >> 3 << 8) + (x & 1) * 16 * ROW_BYTES);
+            };
+            const int vkey = 4 * g + (n >> 2);
+            const unsigned vat = (vkey * ROW_BYTES + ((((n >> 1) & 1) ^ vkey) << 4) + (n & 1) * 8) ^ (CB < 16 ? cg * CB << 5 : 0);
+            auto v_block = [](int x) { return CB == 16 ? x >> 1 | (x & 1) << 3 : x; };
+            auto v_frag = [&](int x) {
+                const int j = v_block(x);
+                const unsigned char* const at = vt + (vat ^ ((j & 7) << 5)) + (j >> 3 << 8);
+                s16x4 a[2];
 #pragma unroll
-                for (int kb = 0; kb < 8; kb++) {
-                    if (RT > 1 && kb == 4) __builtin_amdgcn_sched_barrier(0);
-                    const bf16x8 ka = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(kt + (at ^ (kb << 6))));
+                for (int u = 0; u < 2; u++) a[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + u * 16 * ROW_BYTES));
+                const s16x4 a0 = a[0], a1 = a[1];
+                return __builtin_bit_cast(u32x4, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            u32x4 ring[DEPTH];
 #pragma unroll
-                    for (int t = 0; t < RT; t++) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, bq[t][kb], s[t][u], 0, 0, 0);
-                }
+            for (int x = 0; x < DEPTH; x++) ring[x] = k_frag(x);
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+                    s[t][x & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ring[x % DEPTH]), bq[t][x >> 1], s[t][x & 1], 0, 0, 0);
+                if (x + DEPTH < 16) ring[x % DEPTH] = k_frag(x + DEPTH);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            auto start_v = [&] {
+#pragma unroll
+                for (int x = 0; x < DEPTH && x < CB; x++) ring[x] = v_frag(x);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            if (RT == 1) start_v();                              // (with two row tiles a wavefront the registers are taken until the softmax is done)
             // online softmax on the raw products: lane (row n, group g) holds keys 16 u + 4 g .. + 3
             const bool masked = is_new || key0 + KT > keys;
             u32x2 ph[RT][KT / 16], pl[SPLIT ? RT : 1][KT / 16];
@@ -291,7 +332,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                         for (int i = 0; i < 4; i++) {
                             const int key = key0 + 16 * u + 4 * g + i;
                             const bool on = is_new ? key < M && (seen >> (key & 63) & 1) : key < keys;
-                            s[t][u][i] = on ? s[t][u][i] : NEG;
+                            s[t][u][i] = on ? s[t][u][i] : -INFINITY;
                         }
                 }
                 float mx = fmaxf(s[t][0][0], s[t][0][1]);
@@ -310,7 +351,6 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], SCALE_LOG2E, -mc));
-                        if (masked && s[t][u][i] <= 0.5f * NEG) p[i] = 0.f;
                         if constexpr (SPLIT) sum += p[i];
                     }
                     const u32x2 h = {pack2_bf(p[0], p[1]), pack2_bf(p[2], p[3])};
@@ -318,7 +358,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                     if constexpr (SPLIT)
                         pl[t][u] = u32x2{pack2_bf(p[0] - lo_bf(h[0]), p[1] - hi_bf(h[0])), pack2_bf(p[2] - lo_bf(h[1]), p[3] - hi_bf(h[1]))};
                     else
-                        sum += (lo_bf(h[0]) + hi_bf(h[0])) + (lo_bf(h[1]) + hi_bf(h[1]));
+                        sum = pair_sum(h[1], pair_sum(h[0], sum));
                 }
                 l_run[t] = l_run[t] * corr + sum;                // this lane's share; summed over g at the end
                 m_run[t] = m_new;
@@ -327,20 +367,12 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                     for (int j = 0; j < CB; j++) O[t][j] *= corr;
                 }
             }
-            // transposing load: lane (n, g) points at key 4 g + n / 4, columns 4 (n % 4) .. + 3 of the block, and receives keys 4 g .. + 3 of column n.  Two of them are
-            // the A operand when the 32 keys are enumerated as 16 (e >> 2) + 4 g + (e & 3), in which order the lane holds its probabilities.
-            const int vkey = 4 * g + (n >> 2);
-            const unsigned vat = vkey * ROW_BYTES + ((((n >> 1) & 1) ^ vkey) << 4) + (n & 1) * 8;
+            if (RT > 1) start_v();
 #pragma unroll
-            for (int j = 0; j < CB; j++) {
-                if (RT > 1 && j % 4 == 0) __builtin_amdgcn_sched_barrier(0);    // (at most four column blocks' fragments in registers at a time)
-                s16x4 a[2];
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    a[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4*)(vt + (vat ^ ((cg * CB + j) << 5)) + u * 16 * ROW_BYTES));
-                const s16x4 a0 = a[0], a1 = a[1];
-                const bf16x8 av = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int x = 0; x < CB; x++) {
+                const int j = v_block(x);
+                const bf16x8 av = __builtin_bit_cast(bf16x8, ring[x % DEPTH]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
                     const u32x4 hp = {ph[t][0][0], ph[t][0][1], ph[t][1][0], ph[t][1][1]};
@@ -350,6 +382,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                         O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, lp), O[t][j], 0, 0, 0);
                     }
                 }
+                if (x + DEPTH < CB) ring[x % DEPTH] = v_frag(x + DEPTH);
             }
         }
         const Visit next = find_visit(v.sg + 1);
