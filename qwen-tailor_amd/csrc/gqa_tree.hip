@@ -212,22 +212,51 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
 
     Visit v = find_visit(sg);
     if (v.sg < 0) return;
+    // Q^T: lane (row n, group g) holds q[row n][32 kb + 8 g .. + 8] of each row tile (rows past the last token repeat it; they are not stored).
+    // Up to 64 rows come by way of the tile buffer that is not in use yet, ahead of the tiles: the wait for them leaves the tiles in flight (a load into registers is
+    // the compiler's to wait for, which knows nothing of the tiles behind it and waits for those too).
+    constexpr bool STAGE_Q = ROWS <= 64;
     bf16x8 bq[RT][8];
-    auto load_q = [&] {                                          // Q^T: lane (row n, group g) holds q[row n][32 kb + 8 g .. + 8] of each row tile
-        const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+    auto ask_q = [&](const Visit& v) {
+        if constexpr (STAGE_Q) {
+            const unsigned buf = lds0 + (unsigned)((v.t0 + AHEAD) & (BUFS - 1)) * (2 * TILE_BYTES);
+            const bf16_t* const qs = q + ((size_t)(v.sg / AKV) * M * AH + v.sg % AKV * GQA) * AD;
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int tok = min((rg * RT + t) * 4 + n / GQA, M - 1);          // (rows past the last token repeat it; they are not stored)
-            const u32x4* qr = reinterpret_cast<const u32x4*>(q + ((size_t)(v.sg / AKV * M + tok) * AH + v.sg % AKV * GQA + n % GQA) * AD);
-#pragma unroll
-            for (int kb = 0; kb < 8; kb++) bq[t][kb] = __builtin_bit_cast(bf16x8, qr[kb * 4 + g]);
+            for (int i = 0; i < ROWS / 2 / WAVES; i++) {
+                const int r = 2 * (w + WAVES * i) + (lane >> 5);
+                const unsigned off = (unsigned)((min(r / GQA, M - 1) * AH + r % GQA) * ROW_BYTES) + 16 * ((lane & 31) ^ (r & 15));
+                lds_dma16_at(qs, off, __builtin_amdgcn_readfirstlane(buf + (unsigned)(w + WAVES * i) * (2 * ROW_BYTES)));
+            }
         }
     };
-    load_q();
+    auto load_q = [&] {
+        const int ln = opaque(lane), n = ln & 15, g = ln >> 4;
+        if constexpr (STAGE_Q) {
+            const int later = min(v.t1 - v.t0, AHEAD);           // tiles in flight behind the rows
+            if (later == 3) wait_vmem<3 * PER_TILE>();
+            else if (later == 2) wait_vmem<2 * PER_TILE>();
+            else wait_vmem<PER_TILE>();
+            barrier();
+            const unsigned char* const qt = tile_s + ((v.t0 + AHEAD) & (BUFS - 1)) * (2 * TILE_BYTES) + (rg * 16 + n) * ROW_BYTES;
+#pragma unroll
+            for (int kb = 0; kb < 8; kb++) bq[0][kb] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qt + ((((4 * kb + g) ^ n)) << 4)));
+        } else {
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const int tok = min((rg * RT + t) * 4 + n / GQA, M - 1);
+                const u32x4* qr = reinterpret_cast<const u32x4*>(q + ((size_t)(v.sg / AKV * M + tok) * AH + v.sg % AKV * GQA + n % GQA) * AD);
+#pragma unroll
+                for (int kb = 0; kb < 8; kb++) bq[t][kb] = __builtin_bit_cast(bf16x8, qr[kb * 4 + g]);
+            }
+        }
+    };
+    ask_q(v);
+    if (!STAGE_Q) load_q();
     __builtin_amdgcn_sched_barrier(0);
     for (int i = 0; i < AHEAD; i++)
         if (v.t0 + i < v.t1) issue(v, v.t0 + i);
     while (true) {
+        if (STAGE_Q) load_q();
         const int pool_tiles = (v.p0 + KT - 1) / KT;
         const bool has_new = v.t1 > pool_tiles;
         if (has_new && w == 0) {
@@ -387,6 +416,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         }
         const Visit next = find_visit(v.sg + 1);
         __syncthreads();                                         // everyone is done with the tiles, and has said what is not finite
+        if (next.sg >= 0) ask_q(next);
         if (next.sg >= 0)
             for (int i = 0; i < AHEAD; i++)
                 if (next.t0 + i < next.t1) issue(next, next.t0 + i);
@@ -424,7 +454,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         if (next.sg < 0) break;
         __syncthreads();                                         // (the next visit clears what this one has collected)
         v = next;
-        load_q();
+        if (!STAGE_Q) load_q();
     }
 }
 
