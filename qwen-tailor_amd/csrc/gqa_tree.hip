@@ -13,6 +13,10 @@
 // Eight wavefronts: each takes row tiles of its own; where there are fewer than eight, CG of them share a row tile's scores and take 256 / CG columns of O
 // each.  (Key halves instead would need half the score products, but a partial result each.)
 // A visit to a segment is prepared while the one before is finished: its first tiles are asked for ahead of the stores of the partial result.
+//
+// Measured, both launches: 1 sequence x 7 tokens on 300 keys 11.5 us (launches, then slots, segment, rows and tiles one after the other); 16 x 16 on 1024 - 8192 keys 40 us
+// (151 MB of cache; the tiles stream at 6 TB/s, the first has landed after 6 us); 8 x 64 on 8192 - 32768 keys 122.5 us (336 MB, 86 GFLOP: matrix units
+// busy 40 % of the time at 1.85 GHz, beside them 140 vector instructions a tile and wavefront, and 70 MB of partial results written and read).
 #include "tree.h"
 
 using namespace qt;
