@@ -249,7 +249,7 @@ int qt_blit_fill_batch(void* const* dst, const void* const* src, const long* met
  * A drafted tree: sequence b drafts M tokens (1 <= M <= 64), parents [B,M] int32 is the index of a token's parent among them, smaller than its own,
  * or -1: a child of the sequence's last committed token (anything else counts as -1).  A sequence that drafts fewer pads its rows with
  * -1; no other token sees them.  Row b*M + j is token j.  Values of a token that are not finite reach no row that does not descend from it;
- * the token's own row and its descendants' become NaN.  Output rows of skipped sequences are zero.
+ * the token's own row and its descendants' become NaN (in the attention a key whose score is -inf takes no weight).  Output rows of skipped sequences are zero.
  *
  * qt_gdn_tree_step: the GatedDeltaNet step of the M tokens, every token from the state and conv window that its parent leaves (the outputs of
  * qt_gdn_verify_step for a chain, up to the order of sums).  proj [B*M,8224]; pools, slots and pos as for qt_gdn_decode_step; the pools are only read and

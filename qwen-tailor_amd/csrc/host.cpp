@@ -998,8 +998,10 @@ PyObject* attn_layer_bt(PyObject* const* a) {
     }));
 }
 
-// The layers of a stack's pools (lists of tensors, all of one shape), checked, as tables of pointers
+// The layers of a stack's pools (lists of tensors, all of one shape), checked, as tables of pointers (and held: another thread may change the lists while the
+// interpreter's lock is free)
 struct PoolList {
+    std::vector<Tensor> held;
     std::vector<float*> ssm;
     std::vector<void*> conv, kv;
     int64_t n_slots = -1, Lmax = 0;
@@ -1012,6 +1014,7 @@ struct PoolList {
             n_slots = s.size(0);
             const Tensor& c = dev(pc[i], BF16, "conv", {n_slots * 2, 3, CD});
             on(s, "ssm"), on(c, "conv");
+            held.push_back(s), held.push_back(c);
             ssm.push_back(s.data_ptr<float>());
             conv.push_back(c.data_ptr());
         }
@@ -1019,6 +1022,7 @@ struct PoolList {
             const Tensor& t = dev(i & 1 ? pv[i / 2] : pk[i / 2], BF16, i & 1 ? "V" : "K", {n_slots, 2, i ? Lmax : ANY, 256});
             n_slots = t.size(0), Lmax = t.size(2);
             on(t, i & 1 ? "V" : "K");
+            held.push_back(t);
             kv.push_back(t.data_ptr());
         }
         if (n_slots < 0) value_error("pools: no layers");
@@ -1041,7 +1045,7 @@ PyObject* tree_commit(PyObject* const* a) {
     int64_t M = a[12] == Py_None ? 0 : integer(a[12]);
     std::vector<const void*> proj, cw;
     std::vector<const float*> A, dtb;
-    std::vector<Tensor> held;                                    // (what had to be converted)
+    std::vector<Tensor> held;
     for (size_t i = 0; i < n; i++) {
         const Tensor& t = dev(projs[i], BF16, "proj", {ANY, PW});
         if (M == 0 && B > 0) M = t.size(0) / B;
@@ -1049,7 +1053,7 @@ PyObject* tree_commit(PyObject* const* a) {
         const Tensor& w = flat_conv_w(cws[i]);
         const Tensor Ai = f32(As[i], "A_log", HV), di = f32(dts[i], "dt_bias", HV);
         on(t, "proj"), on(w, "conv_w"), on(Ai, "A_log"), on(di, "dt_bias");
-        held.push_back(Ai), held.push_back(di);
+        held.push_back(t), held.push_back(w), held.push_back(Ai), held.push_back(di);
         proj.push_back(t.data_ptr()), cw.push_back(w.data_ptr()), A.push_back(Ai.data_ptr<float>()), dtb.push_back(di.data_ptr<float>());
     }
     if (B == 0) Py_RETURN_NONE;

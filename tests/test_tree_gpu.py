@@ -519,6 +519,91 @@ def test_a_round_of_drafting_leaves_what_decode_steps_would(dev):
         check_tensors_equal("o again", go, o)
 
 
+def both_layers(case, P, dev):
+    """one tree step of a recurrent and an attention layer, as a function of nothing"""
+    import qwen_tailor_amd as qt
+    proj, qkv, p, qn, kn, slots, pos, parents = case
+    return (qt.batch_tree.deltanet_bt(proj, P.conv[0], *p, P.ssm[0], slots, pos, parents), qt.batch_tree.attn_layer_bt(qkv, qn, kn, P.K[0], P.V[0], slots, pos, parents),
+            qt.batch_tree.attn_bt(qkv[:, :2048].reshape(-1, 8, 256).contiguous(), qkv[:, 4096:4608].reshape(-1, 2, 256).contiguous(),
+                                  qkv[:, 4608:].reshape(-1, 2, 256).contiguous(), P.K[0], P.V[0], slots, pos, parents))
+
+
+def layer_case(gen, seed, B, M, Lmax, dev):
+    rng = np.random.default_rng(seed)
+    r = lambda *s: torch.empty(s, dtype=BF16, device=dev).normal_(generator=gen)  # noqa: E731
+    i = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    qn, kn = ((1 + 0.1 * r(256).float()).to(BF16) for _ in range(2))
+    return r(B * M, PW), r(B * M, 5120), params(gen, dev), qn, kn, i(rng.permutation(B + 1)[:B]), i(rng.integers(0, Lmax - M, B)), i(trees(rng, B, M, "random"))
+
+
+SHAPES = [(1, 7, 100), (3, 24, 700), (2, 64, 300)]
+
+
+def test_calls_from_threads_on_streams_of_their_own(dev):
+    """the same bits as one after the other: no scratch in common between streams"""
+    import threading
+    gen = torch.Generator(dev).manual_seed(21)
+    cases = [(layer_case(gen, k, B, M, L, dev), PoolSet(gen, 1, 1, B + 1, L, dev)) for k, (B, M, L) in enumerate(SHAPES)]
+    want = [both_layers(c, P, dev) for c, P in cases]
+    torch.cuda.synchronize()
+    got, errors = [None] * len(cases), []
+
+    def work(k):
+        try:
+            with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.Stream()):
+                got[k] = [both_layers(*cases[k], dev) for _ in range(10)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for w, g in zip(want, got):
+        for again in g:
+            for a, b in zip(again, w):
+                check_tensors_equal("out", a, b)
+
+
+def test_graphs_captured_on_one_stream_replayed_side_by_side(dev):
+    """each graph has scratch of its own: replayed on two streams at once, with eager calls between, the outputs are those of eager calls"""
+    gen = torch.Generator(dev).manual_seed(22)
+    cases = [(layer_case(gen, k, B, M, L, dev), PoolSet(gen, 1, 1, B + 1, L, dev)) for k, (B, M, L) in enumerate(SHAPES)]
+    want = [both_layers(c, P, dev) for c, P in cases]
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c, P in cases:
+            both_layers(c, P, dev)
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(both_layers(c, P, dev))
+            graphs.append(g)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    for _ in range(4):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+            graphs[1].replay()
+        with torch.cuda.stream(other):
+            graphs[2].replay()
+        eager = both_layers(*cases[1], dev)                      # (the pool rows that it writes are those that the graph writes: the same values)
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            for a, b in zip(o, w):
+                check_tensors_equal("replayed", a, b)
+        for a, b in zip(eager, want[1]):
+            check_tensors_equal("eager", a, b)
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------------
 
 def test_refusals(dev):
