@@ -14,7 +14,7 @@
 // each.  (Key halves instead would need half the score products, but a partial result each.)
 // A visit to a segment is prepared while the one before is finished: its first tiles are asked for ahead of the stores of the partial result.
 //
-// Measured, both launches: 1 sequence x 7 tokens on 300 keys 11.5 us (launches, then slots, segment, rows and tiles one after the other); 16 x 16 on 1024 - 8192 keys 40 us
+// Measured, both launches: 1 sequence x 7 tokens on 300 keys 11.7 us (launches, then slots, segment, rows and tiles one after the other); 16 x 16 on 1024 - 8192 keys 40 us
 // (151 MB of cache; the tiles stream at 6 TB/s, the first has landed after 6 us); 8 x 64 on 8192 - 32768 keys 122.5 us (336 MB, 86 GFLOP: matrix units
 // busy 40 % of the time at 1.85 GHz, beside them 140 vector instructions a tile and wavefront, and 70 MB of partial results written and read).
 #include "tree.h"
@@ -34,6 +34,7 @@ constexpr int KT = 32, ROW_BYTES = AD * 2, TILE_BYTES = KT * ROW_BYTES;        /
 constexpr int BUFS = 4, AHEAD = BUFS - 1, WAVES = 8, THREADS = 64 * WAVES;
 constexpr float SCALE_LOG2E = 0.0625f * 1.44269504088896f;                     // 256^-0.5 log2(e): the softmax works with powers of two
 constexpr float NEG = -3.0e38f;
+constexpr int LAYER_TOKENS = 16, ROPE_BYTES = 32 * 8;                          // tokens of the layer form; (cos, sin) pairs of a position
 constexpr int MAX_SEG = 2048, MAX_GRID = 1024;
 
 // the larger of two floats in one instruction (the compiler makes three of fmaxf behind a lane exchange, to quiet signalling NaN)
@@ -106,13 +107,67 @@ __device__ __forceinline__ void lds_dma16_at(const void* base, unsigned off, uns
                  : "memory");
 }
 
-// RT row tiles a wavefront, NRG = 8 / CG groups of wavefronts with rows of their own
-template <int RT, int CG>
+// the same with four bytes a lane
+__device__ __forceinline__ void lds_dma4_at(const void* base, unsigned off, unsigned lds) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
+}
+// What qkv_prep does with a q or k row (attn_glue.hip), in place on row r of a tile by 16 lanes: RMS norm with the sum of squares in double, weights, and the rotation of features
+// 0 .. 63 by the pairs of the row's position.  Lane c has pieces c and 16 + c, and returns them in x.
+__device__ __forceinline__ void norm_row(unsigned char* tile, int r, int c, const unsigned char* weights, const unsigned char* pairs, float eps, u32x4 (&x)[2]) {
+    u32x4* const row = reinterpret_cast<u32x4*>(tile + r * ROW_BYTES);
+    x[0] = row[c ^ (r & 15)], x[1] = row[(16 + c) ^ (r & 15)];
+    double ss = 0.0;
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const double lo = (double)lo_bf(x[hf][j]), hi = (double)hi_bf(x[hf][j]);
+            ss = fma(hi, hi, fma(lo, lo, ss));
+        }
+    const float inv = rsqrt_rn((float)row16_sum_d(ss) / (float)AD + eps);
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++) {
+        const u32x4 wt = *reinterpret_cast<const u32x4*>(weights + 256 * hf + 16 * c);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t t = pack2_bf(lo_bf(x[hf][j]) * inv, hi_bf(x[hf][j]) * inv);
+            x[hf][j] = pack2_bf(lo_bf(wt[j]) * lo_bf(t), hi_bf(wt[j]) * hi_bf(t));
+        }
+    }
+    u32x4 o;                                                     // the partners' features: lane c ^ 4 = the half row mirrored, then every quad reversed
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int m = __builtin_amdgcn_update_dpp(0, (int)x[0][j], 0x141, 0xF, 0xF, true);
+        o[j] = (unsigned)__builtin_amdgcn_update_dpp(0, m, 0x1B, 0xF, 0xF, true);
+    }
+    if (c < 8) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const f32x4 cs = *reinterpret_cast<const f32x4*>(pairs + 64 * (c & 3) + 16 * j);
+            const float a0 = lo_bf(x[0][j]) * cs[0], b0 = lo_bf(o[j]) * cs[1], a1 = hi_bf(x[0][j]) * cs[2], b1 = hi_bf(o[j]) * cs[3];
+            x[0][j] = c < 4 ? pack2_bf(a0 - b0, a1 - b1) : pack2_bf(b0 + a0, b1 + a1);
+        }
+    }
+    row[c ^ (r & 15)] = x[0], row[(16 + c) ^ (r & 15)] = x[1];
+}
+
+// RT row tiles a wavefront, NRG = 8 / CG groups of wavefronts with rows of their own.  LAYER: q, k_new and v_new point into qkv rows; norms and rotation of the query
+// rows in the buffer that they come through, those of the new keys in their tile.  Every workgroup of a segment does the former again, which costs less than a launch ahead
+// of this one (layer of 1 x 7 tokens on 300 keys 16.8 -> 14.0 us, 16 x 8 on 2000 31.2 -> 29.4, 16 x 16 38.8 -> 37.7).
+template <int RT, int CG, bool LAYER>
 __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_new,
                                                                const bf16_t* __restrict__ v_new, bf16_t* Kp, bf16_t* Vp,
                                                                const int* __restrict__ slots, const int* __restrict__ pos,
                                                                const int* __restrict__ parents, float* __restrict__ part_o,
-                                                               float* __restrict__ part_ml, int* __restrict__ seg_tab, const Plan plan) {
+                                                               float* __restrict__ part_ml, int* __restrict__ seg_tab, const Plan plan,
+                                                               const bf16_t* __restrict__ q_norm, const bf16_t* __restrict__ k_norm,
+                                                               const float2* __restrict__ rope, float eps) {
+    constexpr int Q_W = LAYER ? QKV_W : AH * AD, Q_HEAD = LAYER ? 2 * AD : AD, NEW_W = LAYER ? QKV_W : AKV * AD;      // row and head strides
     constexpr int NRG = WAVES / CG, ROWS = 16 * RT * NRG, CB = 16 / CG;      // rows; column blocks a wavefront takes
     // P as two bf16 terms (off by 2^-17) while the launch is bound by the cache's bytes.  With two row tiles a wavefront the second product would cost a half
     // more MFMA time: P is rounded once (2^-9 of each weight, the sum is taken of the rounded ones), less than the output's own rounding.
@@ -122,6 +177,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
     __shared__ int seg_start[MAX_SEG + 1];
     __shared__ uint64_t seen_s[TREE_MAX];                        // bit i of entry j: token j sees new key i
     __shared__ unsigned bad_s[2];
+    constexpr int LT = LAYER ? LAYER_TOKENS : 4;
+    __shared__ __align__(1024) unsigned char rope_s[LT * ROPE_BYTES], norm_s[2 * ROW_BYTES];       // pairs of positions pos .. pos + M - 1; weights of q and k
+    __shared__ __align__(256) int parent_s[64], depth_s[64];
     const int M = plan.M, nseg = plan.B * AKV;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int rg = w / CG, cg = w % CG;
@@ -191,7 +249,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         return v;
     };
     auto pool_rows = [&](const Visit& v) { return ((size_t)v.slot * AKV + v.sg % AKV) * plan.Lmax * AD; };
-    auto new_rows = [&](const Visit& v) { return ((size_t)(v.sg / AKV) * M * AKV + v.sg % AKV) * AD; };
+    auto new_rows = [&](const Visit& v) { return (size_t)(v.sg / AKV) * M * NEW_W + v.sg % AKV * AD; };
     // Wavefront w brings the row pairs w and w + 8 of a tile: lane l place l & 31 of row 2 i + (l >> 5)
     constexpr int PAIRS = KT / 2 / WAVES, PER_TILE = 2 * PAIRS;  // and issues so many loads for it
     auto issue = [&](const Visit& v, int t) {
@@ -199,7 +257,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         const int pool_tiles = (v.p0 + KT - 1) / KT;
         const bool is_new = t >= pool_tiles;
         const int key0 = (is_new ? t - pool_tiles : t) * KT, left = (is_new ? M : v.p0) - key0;
-        const size_t at = is_new ? new_rows(v) + (size_t)key0 * (AKV * AD) : pool_rows(v) + (size_t)key0 * AD;
+        const size_t at = is_new ? new_rows(v) + (size_t)key0 * NEW_W : pool_rows(v) + (size_t)key0 * AD;
         const bf16_t *ks = (is_new ? k_new : Kp) + at, *vs = (is_new ? v_new : Vp) + at;
         const int ln = RT > 1 ? opaque(lane) : lane;
 #pragma unroll
@@ -207,7 +265,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
             int r = 2 * (w + WAVES * i) + (ln >> 5);
             const unsigned piece = (ln & 31) ^ (r & 15);
             if (left < KT) r = min(r, left - 1);                 // (a key past the end: the last one instead, its weight is 0)
-            const unsigned off = (unsigned)r * (is_new ? AKV * ROW_BYTES : ROW_BYTES) + 16 * piece;
+            const unsigned off = (unsigned)r * (is_new ? NEW_W * 2 : ROW_BYTES) + 16 * piece;
             const unsigned to = buf + (unsigned)(w + WAVES * i) * (2 * ROW_BYTES);
             lds_dma16_at(ks, off, __builtin_amdgcn_readfirstlane(to));
             lds_dma16_at(vs, off, __builtin_amdgcn_readfirstlane(to + TILE_BYTES));
@@ -221,14 +279,22 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
     // the compiler's to wait for, which knows nothing of the tiles behind it and waits for those too).
     constexpr bool STAGE_Q = ROWS <= 64;
     bf16x8 bq[RT][8];
+    uint64_t seen = 0;                                           // (LAYER) of the lane's token
     auto ask_q = [&](const Visit& v) {
         if constexpr (STAGE_Q) {
             const unsigned buf = lds0 + (unsigned)((v.t0 + AHEAD) & (BUFS - 1)) * (2 * TILE_BYTES);
-            const bf16_t* const qs = q + ((size_t)(v.sg / AKV) * M * AH + v.sg % AKV * GQA) * AD;
+            const bf16_t* const qs = q + (size_t)(v.sg / AKV) * M * Q_W + v.sg % AKV * GQA * Q_HEAD;
+            if constexpr (LAYER) {
+                static_assert(LAYER_TOKENS == 4 * 4, "four positions a wavefront");
+                auto at = [&](const void* x) { return __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(char*)x)); };
+                if (w < 4) lds_dma16_at(rope + (size_t)v.p0 * 32, (unsigned)(min(4 * w + (lane >> 4), M - 1) * ROPE_BYTES + 16 * (lane & 15)), at(rope_s) + 1024 * w);
+                if (w == 4) lds_dma4_at(parents + (size_t)(v.sg / AKV) * M, 4 * min(lane, M - 1), at(parent_s));
+                if (w == 5) lds_dma16_from(reinterpret_cast<const char*>((lane < 32 ? q_norm : k_norm) + 8 * (lane & 31)), at(norm_s));
+            }
 #pragma unroll
             for (int i = 0; i < ROWS / 2 / WAVES; i++) {
                 const int r = 2 * (w + WAVES * i) + (lane >> 5);
-                const unsigned off = (unsigned)((min(r / GQA, M - 1) * AH + r % GQA) * ROW_BYTES) + 16 * ((lane & 31) ^ (r & 15));
+                const unsigned off = (unsigned)(min(r / GQA, M - 1) * Q_W + r % GQA * Q_HEAD) * 2 + 16 * ((lane & 31) ^ (r & 15));
                 lds_dma16_at(qs, off, __builtin_amdgcn_readfirstlane(buf + (unsigned)(w + WAVES * i) * (2 * ROW_BYTES)));
             }
         }
@@ -241,9 +307,22 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
             else if (later == 2) wait_vmem<2 * PER_TILE>();
             else wait_vmem<PER_TILE>();
             barrier();
-            const unsigned char* const qt = tile_s + ((v.t0 + AHEAD) & (BUFS - 1)) * (2 * TILE_BYTES) + (rg * 16 + n) * ROW_BYTES;
+            unsigned char* const qt = tile_s + ((v.t0 + AHEAD) & (BUFS - 1)) * (2 * TILE_BYTES);
+            if constexpr (LAYER) {                               // every row once: 16 lanes each
+                const int p = ln < M ? parent_s[ln] : -1;
+                seen = tree_ancestors((unsigned)p < (unsigned)ln ? p : -1, ln);
 #pragma unroll
-            for (int kb = 0; kb < 8; kb++) bq[0][kb] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qt + ((((4 * kb + g) ^ n)) << 4)));
+                for (int r0 = 0; r0 < ROWS; r0 += THREADS / 16) {
+                    const int r = r0 + 4 * w + g, up = __shfl(__popcll(seen), min(r / GQA, M - 1)) - 1;
+                    u32x4 x[2];
+                    norm_row(qt, r, n, norm_s, rope_s + up * ROPE_BYTES, eps, x);
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                barrier();
+            }
+#pragma unroll
+            for (int kb = 0; kb < 8; kb++)
+                bq[0][kb] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qt + (rg * 16 + n) * ROW_BYTES + ((((4 * kb + g) ^ n)) << 4)));
         } else {
 #pragma unroll
             for (int t = 0; t < RT; t++) {
@@ -266,7 +345,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
         if (has_new && w == 0) {
             const int ln = opaque(lane);
             if (ln < 2) bad_s[ln] = 0;
-            seen_s[ln] = tree_ancestors(tree_parent(parents + (size_t)(v.sg / AKV) * M, ln, M), ln);
+            if constexpr (LAYER) seen_s[ln] = seen, depth_s[ln] = __popcll(seen);
+            else seen_s[ln] = tree_ancestors(tree_parent(parents + (size_t)(v.sg / AKV) * M, ln, M), ln);
         }
         // q is waited for here: in the tile loop the compiler would wait for its loads in every turn, and for the tiles in flight with them
 #pragma unroll
@@ -294,6 +374,15 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
             const bool is_new = tile >= pool_tiles;
             const int key0 = is_new ? (tile - pool_tiles) * KT : tile * KT, keys = is_new ? M : v.p0;
             if (is_new) {
+                if constexpr (LAYER) {                           // the keys take their places in the pool
+                    const int key = threadIdx.x >> 4, c = threadIdx.x & 15;
+                    if (key < M) {
+                        u32x4 x[2];
+                        norm_row(tile_s + (tile & (BUFS - 1)) * (2 * TILE_BYTES), key, c, norm_s + ROW_BYTES, rope_s + (depth_s[key] - 1) * ROPE_BYTES, eps, x);
+                        u32x4* const to = reinterpret_cast<u32x4*>(Kp + pool_rows(v) + (size_t)(v.p0 + key) * AD);
+                        to[c] = x[0], to[16 + c] = x[1];
+                    }
+                }
                 // A new value that is not finite must not reach rows that do not see it (0 times NaN): it becomes 0 here, and rows that do
                 // see its token become NaN at the end.  Rows past the last token become 0.
 #pragma unroll
@@ -449,9 +538,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
             const bf16_t *kn = k_new + new_rows(v), *vn = v_new + new_rows(v);
             for (int i = 64 * w + opaque(lane) + max(v.t0 - pool_tiles, 0) * KT * 32, e = min((v.t1 - pool_tiles) * KT, M) * 32; i < e; i += THREADS) {
                 const int key = i / 32, c = i % 32;
-                const size_t to = (pool_rows(v) + (size_t)(v.p0 + key) * AD) / 8 + c, from = (size_t)key * (AKV * AD / 8) + c;
+                const size_t to = (pool_rows(v) + (size_t)(v.p0 + key) * AD) / 8 + c, from = (size_t)key * (NEW_W / 8) + c;
                 const u32x4 kx = reinterpret_cast<const u32x4*>(kn)[from], vx = reinterpret_cast<const u32x4*>(vn)[from];
-                reinterpret_cast<u32x4*>(Kp)[to] = kx;
+                if (!LAYER) reinterpret_cast<u32x4*>(Kp)[to] = kx;
                 reinterpret_cast<u32x4*>(Vp)[to] = vx;
             }
         }
@@ -528,21 +617,28 @@ inline int grid_size() {
 inline int partial_rows(int M) { return M <= 8 ? 32 : M <= 16 ? 64 : M <= 32 ? 128 : 256; }
 constexpr long SEG_TAB_BYTES = ((MAX_SEG + 1) * 4 + 15) / 16 * 16;
 
+struct Rows {                           // what the attention needs of a layer whose qkv rows it takes as they are (rope: null if it does not)
+    const bf16_t *q_norm = nullptr, *k_norm = nullptr;
+    const float2* rope = nullptr;
+    float eps = 0.f;
+};
 int launch(const void* q, const void* k, const void* v, void* Kp, void* Vp, const int32_t* slots, const int32_t* pos, const int32_t* parents, void* out,
-           const void* gate_rows, void* workspace, int B, int M, int Lmax, int n_slots, hipStream_t stream) {
+           const void* gate_rows, void* workspace, int B, int M, int Lmax, int n_slots, hipStream_t stream, const Rows& raw = {}) {
     const int rows = partial_rows(M), nwg = grid_size();
     const size_t cap = (size_t)nwg + (size_t)B * AKV;
     float* const part_o = (float*)workspace;
     float* const part_ml = part_o + cap * rows * AD;
     int* const seg_tab = reinterpret_cast<int*>(part_ml + cap * rows * 2);
     const Plan plan = {B, M, Lmax, n_slots, 2 + rows / 64, 2};
-#define QT_TREE_ATTN(RT, CG)                                                                                                                       \
-    hipLaunchKernelGGL((attn_tree_kernel<RT, CG>), dim3((unsigned)nwg), dim3(THREADS), 0, stream, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, \
-                       (bf16_t*)Kp, (bf16_t*)Vp, slots, pos, parents, part_o, part_ml, seg_tab, plan)
-    if (M <= 8) QT_TREE_ATTN(1, 4);
-    else if (M <= 16) QT_TREE_ATTN(1, 2);
-    else if (M <= 32) QT_TREE_ATTN(1, 1);
-    else QT_TREE_ATTN(2, 1);
+#define QT_TREE_ATTN(RT, CG, LAYER)                                                                                                                  \
+    hipLaunchKernelGGL((attn_tree_kernel<RT, CG, LAYER>), dim3((unsigned)nwg), dim3(THREADS), 0, stream, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, \
+                       (bf16_t*)Kp, (bf16_t*)Vp, slots, pos, parents, part_o, part_ml, seg_tab, plan, raw.q_norm, raw.k_norm, raw.rope, raw.eps)
+    if (M <= 8 && raw.rope) QT_TREE_ATTN(1, 4, true);
+    else if (M <= 8) QT_TREE_ATTN(1, 4, false);
+    else if (M <= 16 && raw.rope) QT_TREE_ATTN(1, 2, true);
+    else if (M <= 16) QT_TREE_ATTN(1, 2, false);
+    else if (M <= 32) QT_TREE_ATTN(1, 1, false);
+    else QT_TREE_ATTN(2, 1, false);
 #undef QT_TREE_ATTN
     QT_CHECK_LAUNCH();
     const dim3 grid((unsigned)((B * M * AH + 3) / 4));
@@ -602,6 +698,12 @@ int qt_gqa_tree_layer(const void* qkv, const void* q_norm, const void* k_norm, c
     for (const void* p : {qkv, q_norm, k_norm, rope_table, (const void*)Kp, (const void*)Vp, (const void*)out, (const void*)workspace})
         if (!aligned16(p)) return QT_ERR_ALIGN;
     if (workspace_bytes < qt_gqa_tree_layer_workspace_bytes(B, M)) return QT_ERR_WORKSPACE;
+    // Up to 16 tokens (whose query rows fit a tile buffer) and with a table of every position there can be: no launch ahead of the attention
+    if (M <= LAYER_TOKENS && table_positions >= Lmax) {
+        const bf16_t* const rows = (const bf16_t*)qkv;
+        return launch(rows, rows + AH * 2 * AD, rows + (AH * 2 + AKV) * AD, Kp, Vp, slots, pos, parents, out, qkv, workspace, B, M, Lmax, n_slots, stream,
+                      {(const bf16_t*)q_norm, (const bf16_t*)k_norm, (const float2*)rope_table, eps});
+    }
     bf16_t* const q = reinterpret_cast<bf16_t*>((char*)workspace + partial_bytes(B, M));
     bf16_t* const k = q + (size_t)B * M * AH * AD;
     bf16_t* const v = k + (size_t)B * M * AKV * AD;

@@ -194,6 +194,56 @@ def test_attention_layer_of_a_tree(dev, B, M, pos, Lmax, shape):
     check_tensors_equal("V pool", V2, V)
 
 
+@pytest.mark.parametrize("B,M,pos,Lmax,shape", [(2, 7, [300, 0], 320, "random"), (3, 16, [100, 31, 184], 200, "deep"), (2, 24, [64, 5], 100, "random")])
+def test_attention_layer_without_a_whole_table(dev, B, M, pos, Lmax, shape):
+    """the C entry with no table of rotary pairs, or one that ends early: the same bits"""
+    import qwen_tailor_amd as qt
+    c = attn_case(dev, 3 * B + M, B, M, pos, Lmax, shape)
+    g = torch.Generator(dev).manual_seed(M)
+    qkv = torch.empty((B * M, 5120), dtype=BF16, device=dev).normal_(generator=g)
+    qn, kn = ((1 + 0.1 * torch.empty(256, device=dev).normal_(generator=g)).to(BF16) for _ in range(2))
+    i = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    idx = [i(c["slots"]), i(pos), i(c["parents"])]
+    K, V = c["Kp"].clone(), c["Vp"].clone()
+    want = qt.batch_tree.attn_layer_bt(qkv, qn, kn, K, V, *idx)
+    ptr, n = qt._lib.ptr, qt._lib.lib().qt_gqa_tree_layer_workspace_bytes(B, M)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    short = torch.empty((Lmax - 1, 32, 2), device=dev)
+    qt._lib.call("qt_rope_table_build", ptr(short), Lmax - 1, qt._lib.stream())
+    for table, positions in ((None, 0), (short, Lmax - 1), (short, 40)):
+        K2, V2, out = c["Kp"].clone(), c["Vp"].clone(), torch.empty_like(want)
+        qt._lib.call("qt_gqa_tree_layer", ptr(qkv), ptr(qn), ptr(kn), ptr(table), positions, ptr(K2), ptr(V2), *[ptr(t) for t in idx], ptr(out), ptr(ws), n, B, M, Lmax,
+                     K.shape[0], 1e-6, qt._lib.stream())
+        check_tensors_equal("out", out, want)
+        check_tensors_equal("K pool", K2, K)
+        check_tensors_equal("V pool", V2, V)
+
+
+@pytest.mark.parametrize("M", [5, 16])
+def test_attention_layer_keeps_what_is_not_finite_to_its_branch(dev, M):
+    """NaN in a drafted token's q, k or v row, in never written rows and in the rows of a skipped sequence"""
+    import qwen_tailor_amd as qt
+    B, Lmax = 2, 90
+    c = attn_case(dev, M, B, M, [50, 0], Lmax, "binary")
+    g = torch.Generator(dev).manual_seed(M)
+    qkv = torch.empty((B * M, 5120), dtype=BF16, device=dev).normal_(generator=g)
+    qn, kn = ((1 + 0.1 * torch.empty(256, device=dev).normal_(generator=g)).to(BF16) for _ in range(2))
+    i = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    c["slots"][1] = -1
+    run = lambda x, K, V: qt.batch_tree.attn_layer_bt(x, qn, kn, K, V, i(c["slots"]), i([50, 0]), i(c["parents"]))  # noqa: E731
+    clean = run(qkv, c["Kp"].clone(), c["Vp"].clone())
+    assert not bool(clean[M:].any())
+    hit = [j for j in range(M) if 2 in way(c["parents"][0], j)]
+    for cols, touched in ((slice(0, 256), [2]), (slice(4096, 4352), hit), (slice(4608, 4864), hit)):
+        x, K, V = qkv.clone(), c["Kp"].clone(), c["Vp"].clone()
+        K[:, :, 50:], V[:, :, 50:] = NAN, NAN
+        x[2, cols], x[M:] = NAN, NAN
+        y = run(x, K, V)
+        rest = [j for j in range(B * M) if j not in touched]
+        check_tensors_equal(f"{cols}", y[rest], clean[rest])
+        assert bool(y[touched][:, :256].isnan().all()), cols
+
+
 # ---- the recurrent layers ------------------------------------------------------------------------------------------------
 
 def gdn_case(seed, B, M, shape, scale=1.0):
