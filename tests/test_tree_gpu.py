@@ -170,7 +170,9 @@ def test_attention_large_scores_and_long_cache(dev):
         check_tensors_equal("K pool", K, rK)
 
 
-LAYER = [(1, 7, [300], 320, "random"), (3, 16, [100, 0, 777], 800, "binary"), (2, 40, [64, 500], 560, "deep"), (2, 64, [3, 1500], 1600, "random"), (4, 1, [0, 5, 31, 32], 40, "star")]
+LAYER = [(1, 7, [300], 320, "random"), (3, 16, [100, 0, 777], 800, "binary"), (2, 40, [64, 500], 560, "deep"), (2, 64, [3, 1500], 1600, "random"), (4, 1, [0, 5, 31, 32], 40, "star"),
+         (40, 5, list(range(1, 400, 10)), 420, "random"), (33, 12, [33 * (k % 7) for k in range(33)], 300, "deep"), (300, 2, [k % 50 for k in range(300)], 60, "chain"),
+         (1, 16, [20000], 20016, "random")]
 
 
 @pytest.mark.parametrize("B,M,pos,Lmax,shape", LAYER)
