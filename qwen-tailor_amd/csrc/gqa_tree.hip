@@ -15,8 +15,8 @@
 // A visit to a segment is prepared while the one before is finished: its first tiles are asked for ahead of the stores of the partial result.
 //
 // Measured, both launches: 1 sequence x 7 tokens on 300 keys 11.7 us (launches, then slots, segment, rows and tiles one after the other); 16 x 16 on 1024 - 8192 keys 40 us
-// (151 MB of cache; the tiles stream at 6 TB/s, the first has landed after 6 us); 8 x 64 on 8192 - 32768 keys 122.5 us (336 MB, 86 GFLOP: matrix units
-// busy 40 % of the time at 1.85 GHz, beside them 140 vector instructions a tile and wavefront, and 70 MB of partial results written and read).
+// (151 MB of cache; the tiles stream at 6 TB/s, the first has landed after 6 us); 8 x 64 on 8192 - 32768 keys 140 us (336 MB, 86 GFLOP and half of
+// it again for the second term of P: matrix units, beside them 140 vector instructions a tile and wavefront, and 70 MB of partial results written and read).
 #include "tree.h"
 
 using namespace qt;
@@ -49,11 +49,6 @@ __device__ __forceinline__ float max_over_groups(float x) {      // over the lan
     const unsigned mi = larger(a[0], a[1]);
     const auto b = __builtin_amdgcn_permlane16_swap(mi, mi, false, false);
     return __uint_as_float(larger(b[0], b[1]));
-}
-// c + the two bf16 of a word, products and sum in float
-__device__ __forceinline__ float pair_sum(unsigned w, float c) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
 }
 __device__ __forceinline__ float sum_over_groups(float x) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -169,9 +164,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                                                                const float2* __restrict__ rope, float eps) {
     constexpr int Q_W = LAYER ? QKV_W : AH * AD, Q_HEAD = LAYER ? 2 * AD : AD, NEW_W = LAYER ? QKV_W : AKV * AD;      // row and head strides
     constexpr int NRG = WAVES / CG, ROWS = 16 * RT * NRG, CB = 16 / CG;      // rows; column blocks a wavefront takes
-    // P as two bf16 terms (off by 2^-17) while the launch is bound by the cache's bytes.  With two row tiles a wavefront the second product would cost a half
-    // more MFMA time: P is rounded once (2^-9 of each weight, the sum is taken of the rounded ones), less than the output's own rounding.
-    constexpr bool SPLIT = RT == 1;
+    // P takes part as two bf16 terms (off by 2^-16 of a weight).  One term would be off by 2^-8 of each, so an output by 2^-8 sum w |V - o|, which has no bound in terms of the
+    // output: of nearly equal weights on opposite V rows little is left.  The second product costs the launches that the cache's bytes bound nothing, 8 x 64 on
+    // 8192 - 32768 keys 20 us (120 -> 140).
     constexpr int DEPTH = RT == 1 ? 6 : 4;                       // fragments on their way from LDS
     __shared__ __align__(1024) unsigned char tile_s[BUFS * 2 * TILE_BYTES];
     __shared__ int seg_start[MAX_SEG + 1];
@@ -443,7 +438,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
             if (RT == 1) start_v();                              // (with two row tiles a wavefront the registers are taken until the softmax is done)
             // online softmax on the raw products: lane (row n, group g) holds keys 16 u + 4 g .. + 3
             const bool masked = is_new || key0 + KT > keys;
-            u32x2 ph[RT][KT / 16], pl[SPLIT ? RT : 1][KT / 16];
+            u32x2 ph[RT][KT / 16], pl[RT][KT / 16];
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 if (masked) {
@@ -473,14 +468,11 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], SCALE_LOG2E, -mc));
-                        if constexpr (SPLIT) sum += p[i];
+                        sum += p[i];
                     }
                     const u32x2 h = {pack2_bf(p[0], p[1]), pack2_bf(p[2], p[3])};
                     ph[t][u] = h;
-                    if constexpr (SPLIT)
-                        pl[t][u] = u32x2{pack2_bf(p[0] - lo_bf(h[0]), p[1] - hi_bf(h[0])), pack2_bf(p[2] - lo_bf(h[1]), p[3] - hi_bf(h[1]))};
-                    else
-                        sum = pair_sum(h[1], pair_sum(h[0], sum));
+                    pl[t][u] = u32x2{pack2_bf(p[0] - lo_bf(h[0]), p[1] - hi_bf(h[0])), pack2_bf(p[2] - lo_bf(h[1]), p[3] - hi_bf(h[1]))};
                 }
                 l_run[t] = l_run[t] * corr + sum;                // this lane's share; summed over g at the end
                 m_run[t] = m_new;
@@ -499,10 +491,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tree_kernel(const bf16_t* __r
                 for (int t = 0; t < RT; t++) {
                     const u32x4 hp = {ph[t][0][0], ph[t][0][1], ph[t][1][0], ph[t][1][1]};
                     O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, hp), O[t][j], 0, 0, 0);
-                    if constexpr (SPLIT) {
-                        const u32x4 lp = {pl[t][0][0], pl[t][0][1], pl[t][1][0], pl[t][1][1]};
-                        O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, lp), O[t][j], 0, 0, 0);
-                    }
+                    const u32x4 lp = {pl[t][0][0], pl[t][0][1], pl[t][1][0], pl[t][1][1]};
+                    O[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, lp), O[t][j], 0, 0, 0);
                 }
                 if (x + DEPTH < CB) ring[x % DEPTH] = v_frag(x + DEPTH);
             }
