@@ -274,7 +274,7 @@ int qt_gqa_tree_layer(const void* qkv, const void* q_norm, const void* k_norm, c
                       int Lmax, int n_slots, float eps, qt_stream_t stream);
 
 /* The accepted path of each tree becomes part of its sequence, in all layers: path [B,D] (1 <= D <= 64) the indices among the M tokens from the root down,
- * count [B] how many of them (<= 0: nothing happens; more than D count as D).  For each of the n_gdn recurrent layers (tables of
+ * count [B] how many of them (<= 0: nothing happens; more than D or than M count as the smaller of the two, also below).  For each of the n_gdn recurrent layers (tables of
  * device pointers in host memory: proj [B*M,8224], conv_pool, conv_w, A_log, dt_bias, ssm_pool) the state advances in place through those tokens with the
  * bits of as many calls of qt_gdn_decode_step, and the new window goes to conv buffer (pos + count) & 1.  For each of the n_kv K / V pools
  * [n_slots,2,Lmax,256] rows pos + path[j] move to pos + j (all read before the first is written; a path entry that is no token counts as

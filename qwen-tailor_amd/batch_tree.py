@@ -37,7 +37,8 @@ def attn_layer_bt(qkv, q_norm, k_norm, Kp, Vp, slots, pos, parents, eps=1e-6):
 def commit(P, projs, conv_ws, A_logs, dt_biases, slots, pos, path, count, M=None):
     """The accepted path of each tree becomes part of its sequence, in every layer of the pools P (batch.Pools, or any object with its lists conv, ssm, K and
     V).  projs: the projection rows [B*M, 8224] that deltanet_bt was given, one tensor for each recurrent layer; conv_ws, A_logs, dt_biases the
-    layers' parameters.  path int32 [B, D]: indices among the M tokens from the root down, count int32 [B] how many (0: the sequence stays as it is).
+    layers' parameters.  path int32 [B, D]: indices among the M tokens from the root down, count int32 [B] how many (0: the sequence stays as it is; more than D
+    or M count as the smaller of the two).
     In place: states advance with the bits of as many batch.deltanet_b steps, the conv window goes to buffer (pos + count) & 1, K / V rows pos + path[j]
     move to pos + j.  The caller then counts pos + count tokens.  M: tokens a tree, needed only where there is no recurrent layer."""
     L.host.tree_commit(P.conv, P.ssm, P.K, P.V, projs, conv_ws, A_logs, dt_biases, slots, pos, path, count, M)

@@ -342,6 +342,9 @@ __device__ __forceinline__ int path_token(const int* __restrict__ path, int j, i
     return (unsigned)i < (unsigned)M ? i : 0;
 }
 
+// a path has no more entries than there are, and no more than the tree has tokens: rows pos .. pos + M - 1 are what a sequence is known to have room for
+__device__ __forceinline__ int path_length(int count, int M, int D) { return min(count, min(D, M)); }
+
 // a sequence whose slot is none or whose M rows do not fit the K / V pools (Lmax = 0: there are none) is skipped
 __device__ __forceinline__ bool takes_part(int slot, int p0, int M, int n_slots, int Lmax) {
     return (unsigned)slot < (unsigned)n_slots && (Lmax == 0 || (p0 >= 0 && p0 <= Lmax - M));
@@ -361,7 +364,7 @@ __device__ __forceinline__ void gdn_commit(const GdnLayers& layers, int block, c
     const int h = block % HV, b = block / HV % B, layer = block / HV / B;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane >> 4, c = lane & 15;
     const int token = lane < D ? path_token(path + (size_t)b * D, lane, M) : 0;           // entry j of the path in lane j
-    const int slot = slots[b], p0 = pos[b], cnt = min(count[b], D);
+    const int slot = slots[b], p0 = pos[b], cnt = path_length(count[b], M, D);
     if (!takes_part(slot, p0, M, n_slots, Lmax) || cnt <= 0) return;
     const bf16_t* const proj = layers.proj[layer] + (size_t)b * M * PW;
     const bf16_t* const window = layers.conv[layer] + (size_t)(slot * 2 + (p0 & 1)) * 3 * CD;
@@ -466,7 +469,7 @@ __device__ __forceinline__ void kv_commit(const KvLayers& layers, int block, con
     const int head = block % AKV, b = block / AKV % B, pool = block / AKV / B;
     const int lane = threadIdx.x & 63, j0 = threadIdx.x >> 5, c = threadIdx.x & 31;
     const int token = lane < D ? path_token(path + (size_t)b * D, lane, M) : 0;
-    const int slot = slots[b], p0 = pos[b], cnt = min(count[b], D);
+    const int slot = slots[b], p0 = pos[b], cnt = path_length(count[b], M, D);
     if (!takes_part(slot, p0, M, n_slots, Lmax)) return;
     u32x4* const base = reinterpret_cast<u32x4*>(layers.pool[pool] + (((size_t)slot * AKV + head) * Lmax + p0) * AD) + c;
     u32x4 v[TREE_MAX / 8];

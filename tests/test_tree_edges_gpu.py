@@ -1,9 +1,10 @@
-"""Drafted trees (batch_tree) where they can go wrong without the random cases of test_tree_gpu.py showing it: outputs in which opposite values cancel."""
+"""Drafted trees (batch_tree) where they can go wrong without the random cases of test_tree_gpu.py showing it: outputs in which opposite values cancel,
+paths that claim more tokens than there are."""
 import numpy as np
 import pytest
 import torch
 
-from tests.test_tree_gpu import attn_run, trees, way
+from tests.test_tree_gpu import PoolSet, attn_run, params, trees, way
 from tests.util import *  # noqa: F401,F403
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +56,27 @@ def test_attention_of_values_that_cancel(dev, M, pos):
     ref, a, most = attention64(c)
     over = (o.cpu().double() - ref).abs() / attention_bound(c, ref, a, most)
     assert float(over.max()) <= 1.0, f"{float(over.max()):.2f} of the bound"
+
+
+@pytest.mark.parametrize("M,D", [(6, 20), (1, 64), (9, 10), (20, 6)])
+def test_commit_of_counts_beyond_the_tree(dev, M, D):
+    """count > M, count > D, at the end of the pool: what count = min(D, M) does; the rows, heads and slots behind stay as they are"""
+    import qwen_tailor_amd as qt
+    gen = torch.Generator(dev).manual_seed(M)
+    B, Lmax, most = 3, 2 * M + 5, min(D, M)
+    P = PoolSet(gen, 1, 2, B, Lmax, dev)
+    proj, p = torch.empty((B * M, PW), dtype=BF16, device=dev).normal_(generator=gen), params(gen, dev)
+    i = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    path, slots, pos = i(np.random.default_rng(M).integers(0, M, (B, D))), i([2, 0, 1]), i([Lmax - M, Lmax - M, 1])
+    got, want = P.clone(), P.clone()
+    for pools, count in ((want, [most] * B), (got, [most + 1, 2 ** 31 - 1, max(M, D)])):
+        qt.batch_tree.commit(pools, [proj], [p[0]], [p[1]], [p[2]], slots, pos, path, i(count))
+    for name in ("conv", "ssm", "K", "V"):
+        for a, b in zip(getattr(got, name), getattr(want, name)):
+            check_tensors_equal(name, a, b)
+    for name in ("K", "V"):
+        for a, old in zip(getattr(got, name), getattr(P, name)):
+            for s, n in zip(slots.tolist(), pos.tolist()):
+                check_tensors_equal(f"{name}: rows before", a[s, :, :n], old[s, :, :n])
+                check_tensors_equal(f"{name}: rows behind", a[s, :, n + most:], old[s, :, n + most:])
+                check_tensors_equal(f"{name}: rows moved", a[s, :, n:n + most], old[s][:, (n + path[slots.tolist().index(s), :most]).long()])
