@@ -183,16 +183,17 @@ PyObject* wrap(std::initializer_list<Tensor> ts) {
 }
 
 // ---- buffers that outlive a call ----------------------------------------------------------------------------------------
-// Never destroyed: at interpreter exit the allocator that owns their memory may be gone already.  A buffer that is outgrown is
+// Never destroyed: at interpreter exit the allocator that owns their memory may be gone already.  A table that is outgrown is
 // kept: a HIP graph captured earlier replays with its address.
 std::vector<Tensor>& retired() {
     static auto* v = new std::vector<Tensor>;
     return *v;
 }
 // Scratch memory for a kernel's partial results (the C ABI never allocates): one buffer per (purpose, device, stream), because
-// launches on different streams may overlap.  `first`: size of the first allocation, so that growth is rare.  Under HIP graph capture
-// it is memory of the graph, free for the next call once this one has been recorded: graphs captured on one stream may be replayed
-// side by side, and beside eager calls.
+// launches on different streams may overlap.  `first`: size of the first allocation; a buffer that is outgrown is followed by one at least half as
+// large again, so growth is rare, and goes back to the allocator, which gives it out again on the same stream only, behind the launches that still
+// use it.  Under HIP graph capture it is memory of the graph, free for the next call once this one has been recorded: graphs captured on one
+// stream may be replayed side by side, and beside eager calls.
 // The launches of one call must follow each other on their stream: a call holds `busy` over them, so that another thread that uses the
 // same stream (its buffer, then) does not come in between.  It is taken without the GIL.
 struct Scratch {
@@ -219,9 +220,9 @@ Scratch workspace(int purpose, const Tensor& like, long bytes, long first) {
     static auto* m = new std::map<std::tuple<int, int, void*>, Kept>;
     Kept& k = (*m)[{purpose, (int)like.device().index(), stream()}];
     if (!k.buf.defined() || k.buf.numel() < bytes) {
-        Tensor larger = unlocked([&] { return empty({std::max(bytes, first)}, U8, like); });
-        if (k.buf.defined()) retired().push_back(k.buf);         // (also one that another thread has made meanwhile)
-        k.buf = larger;
+        const long more = k.buf.defined() ? k.buf.numel() + k.buf.numel() / 2 : first;
+        Tensor larger = unlocked([&] { return empty({std::max(bytes, more)}, U8, like); });
+        if (!k.buf.defined() || k.buf.numel() < larger.numel()) k.buf = larger;      // (another thread may have made one meanwhile)
     }
     return {k.buf, &k.busy};
 }
