@@ -286,7 +286,8 @@ int qt_tree_commit(const void* const* proj, void* const* conv_pool, const void* 
 
 /* Beam search's selection.  logits: G sequences x W beams x V (dtype 0 bf16, 1 fp16, 2 f32), element strides stride_g, stride_w, the vocabulary contiguous;
  * scores [G,W] the beams' log-probabilities.  Candidate (w, t) scores scores[w] + logits[w][t] - log sum exp logits[w]; the n largest of a
- * sequence go to out_scores, out_parents (w) and out_tokens (t) [G,n] in falling order, equal ones by the lower w V + t.  A candidate whose score is -inf
+ * sequence go to out_scores, out_parents (w) and out_tokens (t) [G,n] in falling order, equal ones by the lower w V + t (log sum exp is
+ * known to 1e-6: candidates of two beams that lie closer may change places, those of one beam never do).  A candidate whose score is -inf
  * or NaN is none; places that are left over get -inf, -1, -1.  W, n <= 64, G W <= 65535.  Workspace: qt_beam_select_workspace_bytes, 16-byte
  * aligned. */
 long qt_beam_select_workspace_bytes(long G, int W, int V, int n, int elem_size);

@@ -2,7 +2,7 @@
 //
 // Selection: with l_w = log sum_t exp(x[w][t]) the score of candidate (w, t) is scores[w] + x[w][t] - l_w; wanted are the n largest of a sequence's
 // W V candidates, equal ones by the lower index w V + t.  The logits are read once: a launch over slices of the vocabulary keeps, per slice,
-// its n largest logits and its part (maximum, sum) of l_w; a second launch joins the slices of a sequence's beams.
+// its n largest logits and its part (reference point, sum) of l_w; a second launch joins the slices of a sequence's beams.
 #include "qt_common.h"
 #include <algorithm>
 #include <type_traits>
@@ -18,6 +18,8 @@ constexpr int SELECT_MAX = 64;          // beams of a sequence, and candidates t
 constexpr int WAVE_CAP = 256;           // candidates a wavefront holds before it keeps the best n of them
 constexpr int NO_INDEX = 0x7fffffff;
 constexpr float LOG2E = 1.44269504088896f;
+// The reference point of the exponentials follows a maximum that is higher by more: a few times a row, and the arguments of the largest terms stay small
+constexpr float REFERENCE_LAG = 1.f;
 
 __device__ __forceinline__ float as_float(bf16_t v) { return bf2f(v); }
 __device__ __forceinline__ float as_float(f16 v) { return (float)v; }
@@ -45,13 +47,6 @@ __device__ __forceinline__ float wave_max(float v) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float wave_sum(float v) {
-    v = row16_sum(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 // A lower bound of the wavefront's n-th largest value, n <= 64: its highest order bits, two at a time, until just n are left or 16 bits are known
 __device__ __forceinline__ float wave_nth(float x, int n) {
     const unsigned key = order_bits(x);
@@ -71,6 +66,10 @@ __device__ __forceinline__ float wave_nth(float x, int n) {
 struct Cand {                           // a logit and its place in the vocabulary
     float x;
     int t;
+};
+struct Part {                           // a part of l_w: log of sum, plus m
+    double sum;
+    float m;
 };
 __device__ __forceinline__ bool before(float x, int t, const Cand& o) { return x > o.x || (x == o.x && t < o.t); }
 
@@ -144,21 +143,25 @@ __device__ __forceinline__ void unpack_piece(u32x4 v, float (&x)[16 / sizeof(T)]
 // tiles (n different logits are no smaller): of a random row about n candidates a workgroup are left, and almost every logit costs its
 // exponential, a comparison and no more.  A wavefront collects its candidates in LDS; when the list has filled (rising or equal logits), it keeps the best
 // n and raises its threshold.
+// l_w: exponentials and their sum over a lane's part of a tile in float (each is off by 2^-23 and by the rounding of its argument, the sum of 32 by 6.5 2^-24 at most), all
+// sums beyond in double: a wavefront may have a whole row, and added up in float equal logits were 1.7e-6 off over 122 tiles, 1e-5 over 2048.  Of normal rows with deviations
+// 1 - 8 l_w is at most 1.4e-7 off.  (16 x 4 rows of 248320, both launches: 16.6 us, with float sums 16.2)
 template <typename T>
 __global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ logits, long stride_g, long stride_w, unsigned V, int n,
-                                                          unsigned tiles, unsigned per_wave, Cand* __restrict__ best, float2* __restrict__ part) {
+                                                          unsigned tiles, unsigned per_wave, Cand* __restrict__ best, Part* __restrict__ part) {
     constexpr int N = 16 / sizeof(T), TILE = 64 * PIECES;        // pieces a tile
     __shared__ Cand list_s[4][WAVE_CAP], flat_s[256];
     __shared__ int count_s[4];
     __shared__ float thr_s[4];
-    __shared__ float2 ml_s[4];
+    __shared__ Part part_s[4];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const unsigned p = blockIdx.x, slices = gridDim.x, r = blockIdx.z * gridDim.y + blockIdx.y;
     const T* const row = logits + (long)blockIdx.z * stride_g + (long)blockIdx.y * stride_w;
     const unsigned first = min((4 * p + w) * per_wave, tiles), last = min(first + per_wave, tiles);
     Cand* const list = list_s[w];
     int count = 0;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;                                         // the wavefront's reference point
+    double l = 0.0;                                              // this lane's sum of exp(x - m)
     float thr = -INFINITY;                                       // candidates are (x, t) at or before (thr, thr_t)
     int thr_t = NO_INDEX;
     if (first == last && lane == 0) thr_s[w] = -INFINITY;
@@ -181,14 +184,18 @@ __global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ 
                 const float t = wave_nth(top, n);
                 if (lane == 0) thr_s[w] = t;
             }
-            const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new;
+            if (__any(top > m + REFERENCE_LAG)) {
+                const float higher = wave_max(top);
+                if (m > -INFINITY) l *= exp((double)m - (double)higher);             // (otherwise l is 0, or NaN already)
+                m = higher;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < PIECES; i++)
 #pragma unroll
                 for (int e = 0; e < N; e++) sum[e & 3] += __builtin_amdgcn_exp2f((x[i][e] - ref) * LOG2E);        // (x log2 e - ref log2 e would lose bits, or overflow)
-            l = l * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));      // (m = -inf: l is 0, or NaN already)
-            m = m_new;
+            l += (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
         }
         if (tile == first) {                                     // (every wavefront comes by once)
             __syncthreads();
@@ -220,8 +227,8 @@ __global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ 
     }
     // the wavefront's part of l_w
     {
-        const float mm = wave_max(m), ref = mm == -INFINITY ? 0.f : mm, ll = wave_sum(l * __expf(m - ref));
-        if (lane == 0) ml_s[w] = make_float2(mm, ll), count_s[w] = count;
+        const double ll = wave_sum_d(l);
+        if (lane == 0) part_s[w] = Part{ll, m}, count_s[w] = count;
     }
     __syncthreads();
     if (count_s[0] + count_s[1] + count_s[2] + count_s[3] > 256) {
@@ -248,13 +255,15 @@ __global__ __launch_bounds__(256) void select_scan_kernel(const T* __restrict__ 
         if (i < total && (threadIdx.x & 3) == 0 && rank < (float)n) best[out + (int)rank] = mine;
     }
     for (int i = total + threadIdx.x; i < n; i += 256) best[out + i] = Cand{-INFINITY, NO_INDEX};
-    if (threadIdx.x == 0) {
-        float mm = ml_s[0].x;
-        for (int v = 1; v < 4; v++) mm = fmaxf(mm, ml_s[v].x);
-        const float ref = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f;
-        for (int v = 0; v < 4; v++) ll += ml_s[v].y * __expf(ml_s[v].x - ref);
-        part[(long)r * slices + p] = make_float2(mm, ll);
+    if (threadIdx.x < 4) {
+        const Part own = part_s[threadIdx.x];
+        float mm = own.m;
+        mm = fmaxf(mm, dpp_mov<0xB1>(mm));
+        mm = fmaxf(mm, dpp_mov<0x4E>(mm));
+        double ll = own.sum * exp((double)own.m - (double)(mm == -INFINITY ? 0.f : mm));
+        ll += dpp_mov_d<0xB1>(ll);
+        ll += dpp_mov_d<0x4E>(ll);
+        if (threadIdx.x == 0) part[(long)r * slices + p] = Part{ll, mm};
     }
 }
 
@@ -266,10 +275,10 @@ __device__ __forceinline__ bool before(const Scored& a, const Scored& b) { retur
 
 // One workgroup of 16 wavefronts per sequence on the entries of its beams' slices.  Threshold as above: the largest of the wavefronts' n-th largest lane maxima.  What is
 // no smaller goes into one list, a candidate's place is the number of those that come before it; should they not fit (many equal scores), the n
-// places are filled one by one with the best candidate behind the one before.  Scores in double: two beams' candidates may lie closer than floats
-// tell apart.
+// places are filled one by one with the best candidate behind the one before.  Scores in double: floats of this size are 1e-6 apart, so they would change the order within
+// a beam; candidates of two beams keep theirs as far as their l_w is known.
 constexpr int JOIN_WAVES = 16, JOIN_THREADS = 64 * JOIN_WAVES, JOIN_CAP = 1024;
-__global__ __launch_bounds__(JOIN_THREADS) void select_join_kernel(const Cand* __restrict__ best, const float2* __restrict__ part,
+__global__ __launch_bounds__(JOIN_THREADS) void select_join_kernel(const Cand* __restrict__ best, const Part* __restrict__ part,
                                                                    const float* __restrict__ scores, int W, int n, int slices,
                                                                    float* __restrict__ out_s, int* __restrict__ out_w, int* __restrict__ out_t) {
     __shared__ double base_s[SELECT_MAX];                        // scores[v] - log of the beam's sum of exp(x - top_s[v])
@@ -284,15 +293,15 @@ __global__ __launch_bounds__(JOIN_THREADS) void select_join_kernel(const Cand* _
     if ((int)threadIdx.x < entries) c0 = mine_in[threadIdx.x];
     if (threadIdx.x == 0) count_s = 0;
     for (int v = w; v < W; v += JOIN_WAVES) {
-        const float2* pr = part + (g * W + v) * slices;
-        float2 own = {-INFINITY, 0.f};
+        const Part* pr = part + (g * W + v) * slices;
+        Part own = {0.0, -INFINITY};
         if (lane < slices) own = pr[lane];
-        float mm = own.x;
-        for (int i = lane + 64; i < slices; i += 64) mm = fmaxf(mm, pr[i].x);
+        float mm = own.m;
+        for (int i = lane + 64; i < slices; i += 64) mm = fmaxf(mm, pr[i].m);
         mm = wave_max(mm);
         const float ref = mm == -INFINITY ? 0.f : mm;
-        double ll = (double)own.y * exp((double)own.x - (double)ref);
-        for (int i = lane + 64; i < slices; i += 64) ll += (double)pr[i].y * exp((double)pr[i].x - (double)ref);
+        double ll = own.sum * exp((double)own.m - (double)ref);
+        for (int i = lane + 64; i < slices; i += 64) ll += pr[i].sum * exp((double)pr[i].m - (double)ref);
         ll = wave_sum_d(ll);
         if (lane == 0) base_s[v] = (double)scores[g * W + v] - log(ll), top_s[v] = ref;
     }
@@ -454,7 +463,7 @@ extern "C" {
 
 long qt_beam_select_workspace_bytes(long G, int W, int V, int n, int elem_size) {
     if (G < 0 || W < 1 || W > SELECT_MAX || V < 1 || n < 1 || n > SELECT_MAX || (elem_size != 2 && elem_size != 4) || G * W > 65535) return -1;
-    return G == 0 ? 0 : G * W * scan_plan(G * W, V, elem_size).slices * ((long)n * (long)sizeof(Cand) + (long)sizeof(float2));
+    return G == 0 ? 0 : G * W * scan_plan(G * W, V, elem_size).slices * ((long)n * (long)sizeof(Cand) + (long)sizeof(Part));
 }
 
 int qt_beam_select(const void* logits, int dtype, long stride_g, long stride_w, const float* scores, float* out_scores, int32_t* out_parents,
@@ -469,7 +478,7 @@ int qt_beam_select(const void* logits, int dtype, long stride_g, long stride_w, 
     if (workspace_bytes < need) return QT_ERR_WORKSPACE;
     const ScanPlan plan = scan_plan((long)G * W, V, elem);
     const int slices = (int)plan.slices;
-    float2* const part = (float2*)workspace;
+    Part* const part = (Part*)workspace;
     Cand* const best = (Cand*)(part + (size_t)G * W * slices);
     const dim3 grid(plan.slices, (unsigned)W, (unsigned)G);
 #define QT_SCAN(T) hipLaunchKernelGGL((select_scan_kernel<T>), grid, dim3(256), 0, stream, (const T*)logits, stride_g, stride_w, (unsigned)V, n, plan.tiles, \
