@@ -310,7 +310,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void select_join_kernel(const Cand* _
         const Cand c = e == (int)threadIdx.x ? c0 : mine_in[e];
         const int v = (unsigned)e / (unsigned)per_beam;
         const double s = base_s[v] + ((double)c.x - (double)top_s[v]);        // (the difference first: both may be the type's lowest value)
-        return Scored{s == s && c.t != NO_INDEX ? s : -INFINITY, v, c.t};
+        return Scored{(float)s > -INFINITY && c.t != NO_INDEX ? s : -INFINITY, v, c.t};     // (as it is given out: a double may be below every float)
     };
     float top = -INFINITY;
     for (int e = threadIdx.x; e < entries; e += JOIN_THREADS) top = fmaxf(top, (float)entry(e).s);

@@ -1,4 +1,5 @@
-"""Beam search's selection (batch_beam.select) where its sums lose most: long rows of equal logits, thousands of beams."""
+"""Beam search's selection (batch_beam.select) where its sums lose most: long rows of equal logits, thousands of beams,
+scores below every float."""
 import math
 
 import numpy as np
@@ -77,3 +78,20 @@ def test_rising_rows(dev, dtype):
     low = torch.where(torch.arange(V, device=dev) < 25000, torch.finfo(dtype).min, up % 7)
     x = torch.stack([up, up.flip(0), low, low.flip(0)])[None].to(dtype)
     check(x, torch.tensor([[-1.0, -2.0, -600.0, -3.0]], device=dev), 6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scores_below_every_float(dev, dtype):
+    """a score that float32 gives out as -inf is no candidate: its place gets -inf, -1, -1 like any that is left over"""
+    import qwen_tailor_amd as qt
+    big = torch.finfo(dtype).max
+    x = torch.full((1, 2, 700), -big, dtype=dtype, device=dev)
+    x[0, 0, 300], x[0, 1, 5], x[0, 1, 699] = big, 0.0, -1.0
+    s, w, t = qt.batch_beam.select(x, torch.tensor([[-1.0, -2.0]], device=dev), 5)
+    assert w[0, :3].tolist() == [0, 1, 1] and t[0, :3].tolist() == [300, 5, 699]
+    lse = math.log(1 + math.exp(-1.0))
+    assert float((s[0, :3].cpu().double() - torch.tensor([-1.0, -2.0 - lse, -3.0 - lse], dtype=torch.float64)).abs().max()) <= 1e-6
+    # of the second beam the others are at -big, which a float holds; those of the first at -2 big are none
+    assert w[0, 3:].tolist() == [1, 1] and t[0, 3:].tolist() == [0, 1] and bool((s[0, 3:] == -big).all())
+    s, w, t = qt.batch_beam.select(x[:, :1], torch.tensor([[-1.0]], device=dev), 3)
+    assert w.tolist() == [[0, -1, -1]] and t.tolist() == [[300, -1, -1]] and s.tolist() == [[-1.0, -math.inf, -math.inf]]
