@@ -253,8 +253,8 @@ int qt_blit_fill_batch(void* const* dst, const void* const* src, const long* met
  *
  * qt_gdn_tree_step: the GatedDeltaNet step of the M tokens, every token from the state and conv window that its parent leaves (the outputs of
  * qt_gdn_verify_step for a chain, up to the order of sums).  proj [B*M,8224]; pools, slots and pos as for qt_gdn_decode_step; the pools are only read and
- * no token's state is stored (qt_tree_commit advances them).  y [B*M,2048].  k and q of a token take part as bf16, the state as two
- * bf16 terms (2^-17 of an element); a |v| of 2^100 or more counts as not finite.  silu_table as for qt_gdn_conv_prep (null:
+ * no token's state is stored (qt_tree_commit advances them).  y [B*M,2048].  k and q of a token take part as bf16, the state in
+ * all its bits; a |v| of 2^100 or more counts as not finite.  silu_table as for qt_gdn_conv_prep (null:
  * SiLU is evaluated; the same bits). */
 int qt_gdn_tree_step(const void* proj, const void* conv_pool, const void* conv_w, const float* A_log, const float* dt_bias, const float* ssm_pool,
                      const int32_t* slots, const int32_t* pos, const int32_t* parents, const void* silu_table, void* y, int B, int M, int n_slots,

@@ -62,11 +62,12 @@ __device__ __forceinline__ void conv8_silu(const u32x4 (&x)[4], const u32x4 (&ta
 //   rows   : the tokens' q, k and v input rows of this head and the stored window go to LDS directly, each once; a token's conv takes its own row and those of
 //            three ancestors from there.  (Read from memory by every token that needs them, a conv waited for its parent's index, then for four rows.)
 //   S      : lane (column n, group g) loads S[16 w + n][32 kb + 16 eh + 4 g .. + 3]: the B operand of K S^T and Q S^T when a 32-deep block is enumerated in
-//            the order (g, eh, i); k and q are stored in LDS in that order.  S = hi + lo in bf16 (off by 2^-17 of an element); k and q are bf16 already
+//            the order (g, eh, i); k and q are stored in LDS in that order.  S = hi + mid + lo in bf16, exact (two terms leave 2^-17 of an element,
+//            which shows where the products with k or q cancel; the third costs 0.2 us, at 64 tokens 0.6); k and q are bf16 already
 //   K K^T, Q K^T : bf16 MFMA, exact products; L and A in float
 //   (I + L) D = R : blocks of 16: the inverses of the diagonal blocks by forward substitution, the rest as products in float (16x16x4): an
 //            accumulator tile, register r of lane group g = row 4 g + r, is the B operand of step r for the k indices 4 g + r
-// Measured, us: 1 sequence x 7 tokens 6.8 (a string of dependent phases of 1 - 2 thousand clocks), 16 x 16 9.6, 16 x 64 21 (of 40 thousand clocks the conv takes 12,
+// Measured, us: 1 sequence x 7 tokens 7.0 (a string of dependent phases of 1 - 2 thousand clocks), 16 x 16 9.8, 16 x 64 21.7 (of 40 thousand clocks the conv takes 12,
 // whose instructions the bf16 rounding points fix, staging 7, products and solve 15).
 template <int MT, bool TABLE>
 __global__ __launch_bounds__(HEAD_THREADS, 2) void gdn_tree_kernel(const bf16_t* __restrict__ proj, const bf16_t* __restrict__ conv_pool,
@@ -260,24 +261,27 @@ __global__ __launch_bounds__(HEAD_THREADS, 2) void gdn_tree_kernel(const bf16_t*
     for (int I = 0; I < MT; I++) ks[I] = qs[I] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < 4; kb++) {
-        u32x4 hi, lo;
+        u32x4 hi, mid, lo;
 #pragma unroll
         for (int eh = 0; eh < 2; eh++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float a = s[kb][eh][2 * i], c = s[kb][eh][2 * i + 1];
                 const uint32_t hw = pack2_bf(a, c);
-                hi[2 * eh + i] = hw;
-                lo[2 * eh + i] = pack2_bf(a - lo_bf(hw), c - hi_bf(hw));
+                const float ra = a - lo_bf(hw), rc = c - hi_bf(hw);
+                const uint32_t mw = pack2_bf(ra, rc);
+                hi[2 * eh + i] = hw, mid[2 * eh + i] = mw;
+                lo[2 * eh + i] = pack2_bf(ra - lo_bf(mw), rc - hi_bf(mw));
             }
-        const bf16x8 bh = __builtin_bit_cast(bf16x8, hi), bl = __builtin_bit_cast(bf16x8, lo);
+        const bf16x8 terms[3] = {__builtin_bit_cast(bf16x8, lo), __builtin_bit_cast(bf16x8, mid), __builtin_bit_cast(bf16x8, hi)};
 #pragma unroll
         for (int I = 0; I < MT; I++) {
             const bf16x8 ka = frag(k_s, I, kb), qa = frag(q_s, I, kb);
-            ks[I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, bl, ks[I], 0, 0, 0);
-            qs[I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qa, bl, qs[I], 0, 0, 0);
-            ks[I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, bh, ks[I], 0, 0, 0);
-            qs[I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qa, bh, qs[I], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 3; t++) {
+                ks[I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, terms[t], ks[I], 0, 0, 0);
+                qs[I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qa, terms[t], qs[I], 0, 0, 0);
+            }
         }
     }
     __syncthreads();

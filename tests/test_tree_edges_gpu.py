@@ -1,10 +1,11 @@
-"""Drafted trees (batch_tree) where they can go wrong without the random cases of test_tree_gpu.py showing it: outputs in which opposite values cancel,
-paths that claim more tokens than there are."""
+"""Drafted trees (batch_tree) where they can go wrong without the random cases of test_tree_gpu.py showing it: outputs in which opposite values cancel, states of which little
+is left, paths that claim more tokens than there are."""
 import numpy as np
 import pytest
 import torch
 
-from tests.test_tree_gpu import PoolSet, attn_run, params, trees, way
+from oracle import gdn_oracle as O
+from tests.test_tree_gpu import PoolSet, attn_run, gdn_case, gdn_reference, gdn_run, params, trees, way
 from tests.util import *  # noqa: F401,F403
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +81,34 @@ def test_commit_of_counts_beyond_the_tree(dev, M, D):
                 check_tensors_equal(f"{name}: rows before", a[s, :, :n], old[s, :, :n])
                 check_tensors_equal(f"{name}: rows behind", a[s, :, n + most:], old[s, :, n + most:])
                 check_tensors_equal(f"{name}: rows moved", a[s, :, n:n + most], old[s][:, (n + path[slots.tolist().index(s), :most]).long()])
+
+
+@pytest.mark.parametrize("M", [1, 16, 17, 33, 64])
+def test_gdn_step_of_states_that_cancel(dev, M):
+    """rows of the state with two elements whose products with q are opposite, and that two bf16 terms would be 2^-17 off in the same direction: what is left has the precision
+    of a float state.  (Equal tokens, so q is the same for all; beta = 0, so the outputs are gamma S q.)"""
+    c = gdn_case(500 + M, 1, M, "chain")
+    c["proj"][:] = c["proj"][:1]
+    slot, pos = int(c["slots"][0]), int(c["pos"][0])
+    c["conv"][2 * slot + (pos & 1)] = c["proj"][0, :CD]
+    c["proj"][:, 8192:8208], c["proj"][:, 8208:8224] = -60.0, -8.0
+    u = O.conv_silu(c["conv"][2 * slot + (pos & 1)], c["proj"][0, :CD], c["cw"])
+    q, _ = O.normalize_qk(u[:2048].reshape(16, 128), u[2048:4096].reshape(16, 128))
+    q = np.asarray(q, np.float64)
+    two = lambda x: bf(x) + bf(x - bf(x))  # noqa: E731  (exact in float32: the terms do not overlap)
+    rng = np.random.default_rng(M)
+    S = np.zeros((16, 128, 128), np.float32)
+    for h in range(16):
+        big = np.argsort(-np.abs(q[h]))[:16]
+        for v in range(128):
+            i, j = rng.choice(big, 2, replace=False)
+            a = (1.0 + rng.random(4000) * 2 ** -4).astype(np.float32)
+            a = a[np.argmax((a - two(a)) * np.sign(q[h, i]))]                            # q_i times what two terms leave: positive
+            b = (-q[h, i] * a / q[h, j] * (1 + (rng.random(4000) - 0.5) * 2 ** -13)).astype(np.float32)
+            S[h, v, i], S[h, v, j] = a, b[np.argmax((b - two(b)) * np.sign(q[h, j]))]
+    c["ssm"][slot] = S
+    y, ref = to_np(gdn_run(c, dev)).astype(np.float64), gdn_reference(c)
+    # the rounding of the output; six products and their sum in float, and gamma in float of a sum of at most 64 logarithms
+    terms = np.einsum("hvk,hk->hv", np.abs(S.astype(np.float64)), np.abs(q)).ravel()
+    over = np.abs(y - ref) / ((2 ** -8 + 2 ** -20) * np.abs(ref) + 12 * 2 ** -24 * terms)
+    assert over.max() <= 1.0, f"{over.max():.2f} of the bound"
