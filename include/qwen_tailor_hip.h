@@ -248,7 +248,8 @@ int qt_blit_fill_batch(void* const* dst, const void* const* src, const long* met
  *
  * A drafted tree: sequence b drafts M tokens (1 <= M <= 64), parents [B,M] int32 is the index of a token's parent among them, smaller than its own,
  * or -1: a child of the sequence's last committed token (anything else counts as -1).  A sequence that drafts fewer pads its rows with
- * -1; no other token sees them.  Row b*M + j is token j.  Values of a token that are not finite reach no row that does not descend from it;
+ * -1; no other token sees them.  The slots of a call are different from each other, but for those of sequences that pad the batch: they may all point at one
+ * slot, whose contents and whose outputs then mean nothing.  Row b*M + j is token j.  Values of a token that are not finite reach no row that does not descend from it;
  * the token's own row and its descendants' become NaN (in the attention a key whose score is -inf takes no weight).  Output rows of skipped sequences are zero.
  *
  * qt_gdn_tree_step: the GatedDeltaNet step of the M tokens, every token from the state and conv window that its parent leaves (the outputs of
@@ -287,7 +288,7 @@ int qt_tree_commit(const void* const* proj, void* const* conv_pool, const void* 
 /* Beam search's selection.  logits: G sequences x W beams x V (dtype 0 bf16, 1 fp16, 2 f32), element strides stride_g, stride_w, the vocabulary contiguous;
  * scores [G,W] the beams' log-probabilities.  Candidate (w, t) scores scores[w] + logits[w][t] - log sum exp logits[w]; the n largest of a
  * sequence go to out_scores, out_parents (w) and out_tokens (t) [G,n] in falling order, equal ones by the lower w V + t (log sum exp is
- * known to 1e-6: candidates of two beams that lie closer may change places, those of one beam never do).  A candidate whose score is -inf
+ * known to 1e-6: candidates of two beams that lie closer may change places).  A candidate whose score is -inf
  * or NaN is none; places that are left over get -inf, -1, -1.  W, n <= 64, G W <= 65535.  Workspace: qt_beam_select_workspace_bytes, 16-byte
  * aligned. */
 long qt_beam_select_workspace_bytes(long G, int W, int V, int n, int elem_size);

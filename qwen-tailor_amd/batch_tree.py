@@ -2,7 +2,8 @@
 
 batch_spec verifies chains: M tokens a sequence, a state snapshot after each.  Here a sequence's M <= 64 tokens form a tree, given by parents int32 [B, M]
 on the device: the index of a token's parent among the M, smaller than its own, or -1 for a child of the last committed token (anything else counts
-as -1).  A sequence that drafts fewer tokens pads its rows with -1: no other token sees them.  Row b*M + j is token j of sequence b.
+as -1).  A sequence that drafts fewer tokens pads its rows with -1: no other token sees them.  Row b*M + j is token j of sequence b.  The slots of a call
+are different from each other, but for those of sequences that pad the batch: they may all point at the trash slot, and their outputs mean nothing.
 
 A round: the layers run deltanet_bt / attn_layer_bt on the tree, which leave the recurrent state and the conv window as they are and the K / V
 rows of the tree behind the cache; the program picks a path (path int32 [B, D], count int32 [B]); commit takes it into the pools of all layers.

@@ -1,5 +1,5 @@
 """Drafted trees (batch_tree) where they can go wrong without the random cases of test_tree_gpu.py showing it: outputs in which opposite values cancel, states of which little
-is left, paths that claim more tokens than there are."""
+is left, paths that claim more tokens than there are, workgroups that go from one sequence to the next, masks under long caches, padding in a common slot."""
 import numpy as np
 import pytest
 import torch
@@ -112,3 +112,122 @@ def test_gdn_step_of_states_that_cancel(dev, M):
     terms = np.einsum("hvk,hk->hv", np.abs(S.astype(np.float64)), np.abs(q)).ravel()
     over = np.abs(y - ref) / ((2 ** -8 + 2 ** -20) * np.abs(ref) + 12 * 2 ** -24 * terms)
     assert over.max() <= 1.0, f"{over.max():.2f} of the bound"
+
+
+# ---- workgroups with several segments -------------------------------------------------------------------------------------
+
+def visits(dev, B, M, pos):
+    """the most segments (sequence, KV head) that one workgroup of the attention launch takes part in, from the launch's own plan, and how many segments there are"""
+    rows = 32 if M <= 8 else 64 if M <= 16 else 128 if M <= 32 else 256
+    extra, nwg = 2 + rows // 64, torch.cuda.get_device_properties(dev).multi_processor_count
+    size = np.repeat([(n + 31) // 32 + (M + 31) // 32 + extra if n >= 0 else 0 for n in pos], 2)
+    end = np.cumsum(size)
+    per = max(2, -(-int(end[-1]) // nwg))
+    most = 0
+    for w in range(nwg):
+        a, b = w * per, min((w + 1) * per, int(end[-1]))
+        most = max(most, int(((end - size + extra < b) & (end > a) & (size > 0)).sum()))
+    return most, 2 * B
+
+
+def short_caches(B):
+    return [(7 * k) % 40 for k in range(B)]
+
+
+def one_long(B, n):
+    return [n if k == B // 3 else (5 * k) % 33 for k in range(B)]
+
+
+VISITS = [(200, 5, short_caches(200)), (200, 12, short_caches(200)), (300, 16, short_caches(300)), (32, 13, one_long(32, 40000)), (180, 24, short_caches(180)), (32, 20, one_long(32, 50000)),
+          (150, 64, short_caches(150)), (300, 40, short_caches(300)), (32, 50, one_long(32, 60000))]
+
+
+def visit_case(dev, B, M, pos):
+    rng, g = np.random.default_rng(B + M), torch.Generator(dev).manual_seed(B + M)
+    r = lambda *s: torch.empty(s, dtype=BF16, device=dev).normal_(generator=g)  # noqa: E731
+    S, Lmax = B, max(pos) + M
+    pos = np.array(pos, np.int32)
+    slots = rng.permutation(S)[:B].astype(np.int32)
+    pos[4], slots[6] = -1, S + 9                                 # two that are skipped
+    most, segments = visits(dev, B, M, [int(p) if s < S else -1 for p, s in zip(pos, slots)])
+    assert most >= 2, (most, segments)
+    return {"qkv": r(B * M, 5120), "q_norm": r(256), "k_norm": r(256), "Kp": r(S, 2, Lmax, 256), "Vp": r(S, 2, Lmax, 256), "slots": slots, "pos": pos, "parents": trees(rng, B, M, "random")}
+
+
+@pytest.mark.parametrize("B,M,pos", VISITS)
+def test_attention_from_one_sequence_to_the_next(dev, B, M, pos):
+    """workgroups with several visits, at every number of row tiles, with at most 64 segments and with more: against 64 bits, and the layer against attn_bt"""
+    import qwen_tailor_amd as qt
+    c = visit_case(dev, B, M, pos)
+    i = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    skipped = [4, 6]
+    at = np.array([max(int(c["pos"][b]), 0) + len(way(c["parents"][b], j)) - 1 for b in range(B) for j in range(M)])
+    c["q"], c["k"], c["v"] = qt.attention.qkv_prep(c["qkv"], c["q_norm"], c["k_norm"], i(at))
+    c["v"].reshape(B, M, -1)[skipped] = float("nan")
+    o, K, V = attn_run(c, dev)
+    K2, V2 = c["Kp"].clone(), c["Vp"].clone()
+    got = qt.batch_tree.attn_layer_bt(c["qkv"], c["q_norm"], c["k_norm"], K2, V2, i(c["slots"]), i(c["pos"]), i(c["parents"]))
+    want = qt.attention.out_gate(o, c["qkv"]).reshape(B, M, -1)
+    want[skipped] = 0
+    check_tensors_equal("layer", got.reshape(B, M, -1), want)
+    check_tensors_equal("layer: K", K2, K)
+    check_tensors_equal("layer: V", V2, V)
+    assert not bool(o.reshape(B, -1)[skipped].any())
+    keep = [b for b in range(B) if b not in skipped]
+    rows = [b * M + j for b in keep for j in range(M)]
+    for name, pool, new in (("K", K, c["k"]), ("V", V, c["v"])):
+        old = c[name + "p"].clone()
+        for b in keep:
+            old[c["slots"][b], :, c["pos"][b]:c["pos"][b] + M] = new[b * M:(b + 1) * M].transpose(0, 1)
+        check_tensors_equal(name, pool, old)
+    d = {"q": c["q"][rows], "k": c["k"][rows], "v": c["v"][rows], "Kp": c["Kp"], "Vp": c["Vp"], "slots": c["slots"][keep], "pos": c["pos"][keep], "parents": c["parents"][keep]}
+    ref, a, most = attention64(d)
+    over = (o[rows].cpu().double() - ref).abs() / attention_bound(d, ref, a, most)
+    assert float(over.max()) <= 1.0, f"{float(over.max()):.2f} of the bound"
+
+
+@pytest.mark.parametrize("M", [6, 16, 30, 64])
+def test_masks_under_a_long_cache(dev, M):
+    """the new keys carry most of the weight of a row, so that one that is wrongly seen or left out shows, however long the cache is.  (The bound notices: a mistake in the
+    oracle's tree is beyond it in the rows that it concerns.)"""
+    g = torch.Generator(dev).manual_seed(M)
+    r = lambda *s: torch.empty(s, device=dev).normal_(generator=g)  # noqa: E731
+    n, way_in = 20000, r(2, 256)
+    c = {"q": (way_in.repeat_interleave(4, 0) + 0.1 * r(M, 8, 256)).to(BF16), "k": (0.9 * way_in + 0.05 * r(M, 2, 256)).to(BF16), "v": r(M, 2, 256).to(BF16), "Kp": r(2, 2, n + M, 256).to(BF16),
+         "Vp": r(2, 2, n + M, 256).to(BF16), "slots": np.array([1], np.int32), "pos": np.array([n], np.int32), "parents": trees(np.random.default_rng(M), 1, M, "binary")}
+    o, _, _ = attn_run(c, dev)
+    ref, a, most = attention64(c)
+    over = ((o.cpu().double() - ref).abs() / attention_bound(c, ref, a, most)).reshape(M, -1).amax(1)
+    assert float(over.max()) <= 1.0, f"{float(over.max()):.2f} of the bound"
+    wrong = c["parents"].copy()
+    wrong[0, M - 1] = up = (int(wrong[0, M - 1]) + 1) % (M - 1)
+    assert up != int(c["parents"][0, M - 1])
+    bad, a, most = attention64(c, wrong)
+    over = ((o.cpu().double() - bad).abs() / attention_bound(c, bad, a, most)).reshape(M, -1).amax(1)
+    assert float(over[:M - 1].max()) <= 1.0 < float(over[M - 1])
+
+
+# ---- padding --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M", [5, 14, 40])
+def test_padding_sequences_in_a_common_slot(dev, M):
+    """sequences that pad a batch may all point at the pools' last slot, as in a decode step: the others' outputs and slots have the bits that they have when each has a slot of
+    its own"""
+    import qwen_tailor_amd as qt
+    gen, B, Lmax = torch.Generator(dev).manual_seed(M), 6, 130
+    P = PoolSet(gen, 1, 1, 9, Lmax, dev)
+    r = lambda *s: torch.empty(s, dtype=BF16, device=dev).normal_(generator=gen)  # noqa: E731
+    i = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    proj, qkv, p, ones = r(B * M, PW), r(B * M, 5120), params(gen, dev), torch.ones(256, dtype=BF16, device=dev)
+    parents = i(trees(np.random.default_rng(M), B, M, "random"))
+    pos, path, count = i([30, 77, 0, 0, 50, 12]), i([[0, 2, 4]] * B), i([3, 2, 3, 3, 1, 3])
+    runs = []
+    for slots in ([3, 8, 1, 8, 0, 8], [3, 8, 1, 7, 0, 6]):       # 1, 3 and 5 are padding
+        Q, s = P.clone(), i(slots)
+        y = qt.batch_tree.deltanet_bt(proj, Q.conv[0], *p, Q.ssm[0], s, pos, parents)
+        o = qt.batch_tree.attn_layer_bt(qkv, ones, ones, Q.K[0], Q.V[0], s, pos, parents)
+        qt.batch_tree.commit(Q, [proj], [p[0]], [p[1]], [p[2]], s, pos, path, count)
+        real = [0, 2, 4]
+        runs.append([t.reshape(B, M, -1)[real] for t in (y, o)] + [t[:6] for t in (Q.ssm[0], Q.K[0], Q.V[0])] + [Q.conv[0][:12]])
+    for a, b in zip(*runs):
+        check_tensors_equal("the others", a, b)
