@@ -386,6 +386,9 @@ constexpr int KV_WGS = 8;               // workgroups on the rows of one (pool, 
 // UN: places a thread loads before it stores the first; stores are nontemporal.  Bound by HBM: 8 x 4 beams of 24 layers, 1200 rows of the caches, move 1.54 GB in 313 us
 // (4.9 TB/s, a large copy reaches 5.2).  us at 1 x 4 / 8 x 4 beams: one place with plain stores 19.2 / 324, nontemporal stores 18.4 / 314, two places 17.9 /
 // 313, four 19.3 / 317; nontemporal loads lose what two beams take from one parent (22.3 / 312).
+// More beams, one / two / four places: 4 x 8 on 1650 rows 456 / 432 / 420, 1 x 8 206 / 178 / 178, 1 x 6 on 50 rows 25 / 25 / 30, 1 x 16 on 50 rows 97 / 121 / 125, 2 x 16 on 1650 742 / 595 / 487,
+// 1 x 32 on 50 rows 265 / 457, on 1650 859 / 932: beyond 8 beams one place, which is better on short ranges and with 32 beams; long ranges of 16 beams would
+// be faster with more.
 template <int WMAX, int UN>
 __global__ __launch_bounds__(256) void reorder_kernel(const PoolTable pools, const int* __restrict__ slots, const int* __restrict__ parents,
                                                       const int* __restrict__ start, const int* __restrict__ pos, int G, int W, int n_ssm, int n_slots,
@@ -445,9 +448,9 @@ __global__ __launch_bounds__(256) void reorder_kernel(const PoolTable pools, con
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// How a launch cuts its rows: tiles of 4 KiB, tiles a wavefront, workgroups (of four) a row.  Sixteen wavefronts a CU, which all fit, but none without a tile (16 x 4 rows of 248320,
-// us with 8 / 16 / 32 a CU: 23.1 / 17.3 / 18.8; a tile's loads
-// ahead of the one before's arithmetic: no difference).
+// How a launch cuts its rows: tiles of 4 KiB, tiles a wavefront, workgroups (of four) a row.  Sixteen wavefronts a CU, which all fit, but no more than
+// there are tiles (16 x 4 rows of 248320, us with 8 / 16 / 32 a CU: 23.1 / 17.3 / 18.8; a tile's loads ahead of the one before's arithmetic: no difference).  Beyond four rows a CU some of a
+// workgroup's wavefronts have none, of the last workgroup of a row also below; the CU holds other workgroups then (1024 rows 172 us, 2048, two of whose four wavefronts have tiles, 351).
 struct ScanPlan {
     unsigned tiles, per_wave, slices;
 };
@@ -515,7 +518,7 @@ int qt_beam_reorder(float* const* ssm_pool, void* const* conv_pool, int n_gdn, v
         for (int i = 0; i < na; i++) t.ssm[i] = (u32x4*)ssm_pool[a + i], t.conv[i] = (u32x4*)conv_pool[a + i];
         for (int i = 0; i < nk; i++) t.kv[i] = (u32x4*)kv_pool[k + i];
         a += na, k += nk;
-        const int un = W <= 4 ? 2 : W <= 8 ? 2 : 1, per = 256 * un;
+        const int un = W <= 8 ? 2 : 1, per = 256 * un;
         const long blocks = (long)na * G * (SSM_VEC / per + (CONV_VEC + per - 1) / per) + (long)nk * G * AKV * KV_WGS;
         if (blocks > 0x7fffffffl) return QT_ERR_DIM;
 #define QT_REORDER(WM, UN) \

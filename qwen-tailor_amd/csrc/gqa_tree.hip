@@ -14,9 +14,10 @@
 // each.  (Key halves instead would need half the score products, but a partial result each.)
 // A visit to a segment is prepared while the one before is finished: its first tiles are asked for ahead of the stores of the partial result.
 //
-// Measured, both launches: 1 sequence x 7 tokens on 300 keys 11.7 us (launches, then slots, segment, rows and tiles one after the other); 16 x 16 on 1024 - 8192 keys 40 us
-// (151 MB of cache; the tiles stream at 6 TB/s, the first has landed after 6 us); 8 x 64 on 8192 - 32768 keys 140 us (336 MB, 86 GFLOP and half of
-// it again for the second term of P: matrix units, beside them 140 vector instructions a tile and wavefront, and 70 MB of partial results written and read).
+// Measured, us, this launch and the join at the least (profiled): 1 sequence x 7 tokens on 300 keys 8.1 and 3.4 (launches, then slots, segment, rows and tiles one after the other); the layer
+// of 16 x 16 on 1024 - 8192 keys 45.7 and 6.7 (160 MB read: 3.5 TB/s over the launch; the tiles by themselves, without arithmetic, stream at more than 6); 8 x 64 on 8192 - 32768 keys 131
+// and 13.3 (350 MB; a tile takes the matrix units 3070 clocks and the LDS 2050, since each of the eight wavefronts reads all of it; matrix units busy 51 % of the time, beside them 180
+// vector instructions a tile and wavefront; 72 MB of partial results written and read).
 #include "tree.h"
 
 using namespace qt;
@@ -619,6 +620,9 @@ int launch(const void* q, const void* k, const void* v, void* Kp, void* Vp, cons
     float* const part_o = (float*)workspace;
     float* const part_ml = part_o + cap * rows * AD;
     int* const seg_tab = reinterpret_cast<int*>(part_ml + cap * rows * 2);
+    // visit, us with none / as here / twice as many: 1 x 7 on 300 keys 13.4 / 12.0 / 12.2, layer of 16 x 16 on 1024 - 8192 53.6 / 50.6 / 48.0, 32 x 16 on 50 - 400 27.4 / 24.6 / 23.9,
+    // 8 x 64 on 8192 - 32768 157 / 146 / 144, 32 x 64 on 100 - 1000 72.6 / 58.3 / 58.6, 200 x 5 on 20 - 200 36.7 / 33.2 / 33.6, 100 x 64 on 20 - 200 98.7 / 82.2 / 72.5.
+    // min_tiles 1 / 2 / 4 / 8: 1 x 7 on 300 keys 11.2 / 12.0 / 12.6 / 17.4, on 4000 21.9 / 17.4 / 16.0 / 18.6, 1 x 64 on 1000 30.8 / 28.3 / 31.6 / 39.5; in batches all the same.
     const Plan plan = {B, M, Lmax, n_slots, 2 + rows / 64, 2};
 #define QT_TREE_ATTN(RT, CG, LAYER)                                                                                                                  \
     hipLaunchKernelGGL((attn_tree_kernel<RT, CG, LAYER>), dim3((unsigned)nwg), dim3(THREADS), 0, stream, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, \
