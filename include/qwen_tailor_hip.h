@@ -289,7 +289,7 @@ int qt_tree_commit(const void* const* proj, void* const* conv_pool, const void* 
  * scores [G,W] the beams' log-probabilities.  Candidate (w, t) scores scores[w] + logits[w][t] - log sum exp logits[w]; the n largest of a
  * sequence go to out_scores, out_parents (w) and out_tokens (t) [G,n] in falling order, equal ones by the lower w V + t (log sum exp is
  * known to 1e-6: candidates of two beams that lie closer may change places).  A candidate whose score is -inf
- * or NaN is none; places that are left over get -inf, -1, -1.  W, n <= 64, G W <= 65535.  Workspace: qt_beam_select_workspace_bytes, 16-byte
+ * (as a float) or NaN is none; places that are left over get -inf, -1, -1.  W, n <= 64, G W <= 65535.  Workspace: qt_beam_select_workspace_bytes, 16-byte
  * aligned. */
 long qt_beam_select_workspace_bytes(long G, int W, int V, int n, int elem_size);
 int qt_beam_select(const void* logits, int dtype, long stride_g, long stride_w, const float* scores, float* out_scores, int32_t* out_parents,

@@ -14,7 +14,7 @@ def select(logits, scores, n):
     two), scores float32 [G, W]: the beams' log-probabilities, -inf for a beam that is none.  Candidate (w, t) scores scores[w] + log_softmax(logits[w])[t].
     Returns scores float32, parents int32 (w) and tokens int32 (t), each [G, n], in falling order, equal scores by the lower w V + t (the log-sum of a
     beam is known to 1e-6: candidates of two beams that lie closer may change places).  A
-    candidate whose score is -inf or NaN is none; places left over get -inf, -1, -1.  W and n up to 64, G W up to 65535."""
+    candidate whose score is -inf (as float32) or NaN is none; places left over get -inf, -1, -1.  W and n up to 64, G W up to 65535."""
     return L.host.beam_select(logits, scores, n)
 
 
