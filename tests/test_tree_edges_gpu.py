@@ -1,5 +1,5 @@
 """Drafted trees (batch_tree) where they can go wrong without the random cases of test_tree_gpu.py showing it: outputs in which opposite values cancel, states of which little
-is left, paths that claim more tokens than there are, workgroups that go from one sequence to the next, masks under long caches, padding in a common slot."""
+is left, paths that claim more tokens than there are, workgroups that go from one sequence to the next, masks under long caches, padding in a common slot, the largest batch."""
 import numpy as np
 import pytest
 import torch
@@ -231,3 +231,36 @@ def test_padding_sequences_in_a_common_slot(dev, M):
         runs.append([t.reshape(B, M, -1)[real] for t in (y, o)] + [t[:6] for t in (Q.ssm[0], Q.K[0], Q.V[0])] + [Q.conv[0][:12]])
     for a, b in zip(*runs):
         check_tensors_equal("the others", a, b)
+
+
+# ---- the largest batch ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M", [3, 16, 17, 64])
+def test_as_many_sequences_as_there_may_be(dev, M):
+    """1024 sequences in one call: attention as that of 16 calls of 64 (its sums are split elsewhere: two roundings of the output apart), recurrent step and commit with their bits"""
+    import qwen_tailor_amd as qt
+    gen, B, Lmax, at = torch.Generator(dev).manual_seed(M), 1024, 40 + M, 64
+    P = PoolSet(gen, 1, 1, B, Lmax, dev)
+    r = lambda *s: torch.empty(s, dtype=BF16, device=dev).normal_(generator=gen)  # noqa: E731
+    i = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    rng = np.random.default_rng(M)
+    proj, qkv, p, ones = r(B * M, PW), r(B * M, 5120), params(gen, dev), torch.ones(256, dtype=BF16, device=dev)
+    slots, pos, parents = i(rng.permutation(B)), i(rng.integers(0, 41, B)), i(trees(rng, B, M, "random"))
+    path, count = i(np.tile(np.arange(min(M, 5)), (B, 1))), i(rng.integers(0, 6, B))
+
+    def run(Q, a, b):
+        rows, s = slice(a * M, b * M), slice(a, b)
+        y = qt.batch_tree.deltanet_bt(proj[rows], Q.conv[0], *p, Q.ssm[0], slots[s], pos[s], parents[s])
+        o = qt.batch_tree.attn_layer_bt(qkv[rows], ones, ones, Q.K[0], Q.V[0], slots[s], pos[s], parents[s])
+        qt.batch_tree.commit(Q, [proj[rows]], [p[0]], [p[1]], [p[2]], slots[s], pos[s], path[s], count[s])
+        return y, o
+
+    one, many = P.clone(), P.clone()
+    y, o = run(one, 0, B)
+    parts = [run(many, a, a + at) for a in range(0, B, at)]
+    check_tensors_equal("y", y, torch.cat([q[0] for q in parts]))
+    for name in ("conv", "ssm", "K", "V"):
+        check_tensors_equal(name, getattr(one, name)[0], getattr(many, name)[0])
+    want = torch.cat([q[1] for q in parts]).float()
+    # o is rounded, then o times the gate: two steps each, and what float sums in another order leave where little is left (values of V are of size 1)
+    assert bool(((o.float() - want).abs() <= 4 * 2 ** -8 * want.abs() + 1e-4).all())
